@@ -146,6 +146,50 @@ int shtb200_spectral_conv(shtb200_plan *analysis, shtb200_plan *synthesis, const
  */
 int shtb200_quadrature(const float *x_dev, const float *lat_weights_dev, float *out_dev, long long nfields, int nlat, int nlon, void *stream);
 
+/* Element types of the entry points below (the transforms above are float32 / complex64 throughout). */
+enum shtb200_dtype { SHTB200_F32 = 0, SHTB200_BF16 = 1, SHTB200_F16 = 2, SHTB200_C64 = 3 };
+enum shtb200_activation { SHTB200_ACT_NONE = 0, SHTB200_ACT_RELU = 1, SHTB200_ACT_SILU = 2, SHTB200_ACT_GELU = 3 /* z Phi(z), by erf */ };
+enum shtb200_norm { SHTB200_NORM_L2 = 0, SHTB200_NORM_INF = 1 };
+
+/*
+ * Group normalisation of `batch` samples of `channels` fields on an nlat x nlon grid in `groups` groups of consecutive
+ * channels, followed by a scale and shift per channel and an activation.  With a_k = lat_weights[k] (any positive scale; NULL: all 1):
+ *   mu = sum a x / sum a,  v = sum a (x - mu)^2 / sum a   over the channels and grid points of a group,
+ *   y = act(weight_c (x - mu) / sqrt(v + eps) + bias_c).
+ * `dtype` is the type of x, y, dy, dx (F32, BF16, F16), `param_dtype` that of weight, bias and their gradients.
+ * channels_last = 0: [batch, channels, nlat, nlon]; 1: [batch, nlat, nlon, channels].  Statistics and sums are float32 or wider.
+ *   forward : y and stats (16 bytes per (sample, group), 16-byte aligned: what the backward pass needs).
+ *   backward: dx, dweight, dbias, each of which may be NULL; the sums over the batch are taken in a fixed order.
+ * x and y (dy and dx) may not overlap.  Workspace: shtb200_group_norm_workspace_bytes(desc, backward) bytes, 256-byte aligned, 0 for a bad
+ * descriptor.  Runs on the calling thread's current device; no synchronisation; may be captured.
+ */
+typedef struct shtb200_group_norm_desc {
+    int batch, channels, groups, nlat, nlon;
+    int dtype, param_dtype, channels_last, activation;
+    float eps;
+} shtb200_group_norm_desc;
+size_t shtb200_group_norm_workspace_bytes(const shtb200_group_norm_desc *desc, int backward);
+int shtb200_group_norm_forward(const shtb200_group_norm_desc *desc, const void *x_dev, const float *lat_weights_dev, const void *weight_dev, const void *bias_dev, void *y_dev,
+                               void *stats_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
+int shtb200_group_norm_backward(const shtb200_group_norm_desc *desc, const void *dy_dev, const void *x_dev, const float *lat_weights_dev, const void *weight_dev, const void *bias_dev,
+                                const void *stats_dev, void *dx_dev, void *dweight_dev, void *dbias_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
+
+/*
+ * Norm over all entries of `count` tensors of any of the element types (SHTB200_NORM_L2: root of the sum of |g|^2, in float64;
+ * SHTB200_NORM_INF: largest |g|), written to *norm_dev; 0 for no entries.  The arrays of pointers, lengths (entries) and types are host
+ * memory and are read before the call returns.  shtb200_clip_grads then writes dst = src * min(1, max_norm / (norm + 1e-6)); dst[i]
+ * may be src[i], otherwise no two of the buffers may share memory where one is written (SHTB200_EINVAL).  Where nothing is to be clipped, tensors in
+ * place are not touched.  A norm that is not finite goes the same way: inf gives the factor 0, NaN gives NaN.
+ * Workspace: shtb200_grad_norm_workspace_bytes(count), 8-byte aligned.  Current device, no synchronisation, may be captured.
+ */
+size_t shtb200_grad_norm_workspace_bytes(int count);
+int shtb200_grad_norm(int count, const void *const *src_dev, const long long *numel, const int *dtype, int norm, float *norm_dev, void *workspace_dev, size_t workspace_bytes,
+                      void *stream);
+int shtb200_clip_grads(int count, const void *const *src_dev, void *const *dst_dev, const long long *numel, const int *dtype, int norm, float max_norm, float *norm_dev,
+                       void *workspace_dev, size_t workspace_bytes, void *stream);
+/* The second half alone: dst = src * min(1, max_norm / (*norm_dev + 1e-6)) with a norm that is given, e.g. one joined over several processes. */
+int shtb200_scale_grads(int count, const void *const *src_dev, void *const *dst_dev, const long long *numel, const int *dtype, float max_norm, const float *norm_dev, void *stream);
+
 /* Introspection used by the tests and the benchmark. */
 int shtb200_plan_info(const shtb200_plan *plan, int *nlat, int *nlon, int *lmax, int *mmax, int *kind, int *engine);
 /* Kernel launches the last shtb200_execute on this plan enqueued. */

@@ -1,0 +1,133 @@
+"""CPU-only checks of the normalisation module and of gradient clipping: construction, buffers, refusals before any device work."""
+
+import copy
+import ctypes
+import math
+import pickle
+
+import numpy as np
+import pytest
+import torch
+
+import torch_harmonics_b200 as th
+from oracle import sht_oracle as orc
+from torch_harmonics_b200 import _lib, build
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build.build()
+    return _lib.load()
+
+
+@pytest.mark.parametrize("grid", ["equiangular", "legendre-gauss", "lobatto"])
+def test_latitude_weights(grid):
+    m = th.GroupNormS2(2, 4, (13, 24), grid=grid)
+    w = th.QuadratureS2((13, 24), grid=grid).quad_weight[0, 0, :, 0].double()
+    assert m.lat_weights.dtype == torch.float32
+    assert np.allclose(m.lat_weights.double().numpy(), (w / w.mean()).numpy(), rtol=1e-6)
+    assert th.GroupNormS2(2, 4, (13, 24), grid=grid, weighted=False).lat_weights is None
+
+
+def test_module_state():
+    m = th.GroupNormS2(2, 4, (13, 24), activation="gelu")
+    assert set(m.state_dict()) == {"weight", "bias"}
+    assert not list(th.GroupNormS2(2, 4, (13, 24), affine=False).parameters())
+    lat = m.lat_weights.clone()
+    for n in (copy.deepcopy(m), pickle.loads(pickle.dumps(m))):
+        assert torch.equal(n.lat_weights, lat) and n.activation == "gelu"
+    m = m.half()
+    assert m.weight.dtype == torch.float16 and m.lat_weights.dtype == torch.float32 and torch.equal(m.lat_weights, lat)
+    assert "num_groups=2" in repr(m)
+
+
+def test_construction_refusals():
+    for bad in (dict(num_groups=3, num_channels=4), dict(num_groups=0, num_channels=4), dict(num_groups=1, num_channels=0)):
+        with pytest.raises(ValueError):
+            th.GroupNormS2(**bad, img_shape=(13, 24))
+    with pytest.raises(ValueError, match="Unknown activation"):
+        th.GroupNormS2(2, 4, (13, 24), activation="tanh")
+    with pytest.raises(ValueError, match="Unknown quadrature mode"):
+        th.GroupNormS2(2, 4, (13, 24), grid="hexagonal")
+    for eps in (-1.0, math.nan):
+        with pytest.raises(ValueError, match="eps"):
+            th.GroupNormS2(2, 4, (13, 24), eps=eps)
+
+
+def test_no_cpu_path():
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        th.GroupNormS2(2, 4, (13, 24))(torch.zeros(1, 4, 13, 24))
+    p = torch.nn.Parameter(torch.ones(3))
+    p.grad = torch.ones(3)
+    for call in (lambda: th.clip_grad_norm_([p], 1.0), lambda: th.clip_by_global_norm([p.grad], 1.0), lambda: th.global_norm(p.grad)):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            call()
+
+
+def test_clipping_arguments():
+    p = torch.nn.Parameter(torch.ones(3))
+    for bad in (1.0, 0.0, 3, -math.inf, math.nan):
+        with pytest.raises(ValueError, match="norm_type"):
+            th.clip_grad_norm_([p], 1.0, norm_type=bad)
+    for bad in (-1.0, math.nan):
+        with pytest.raises(ValueError, match="max_norm"):
+            th.clip_grad_norm_([p], bad)
+        with pytest.raises(ValueError, match="max_norm"):
+            th.clip_by_global_norm([torch.ones(3)], bad)
+    # nothing to clip
+    assert float(th.clip_grad_norm_([p], 1.0)) == 0.0 and float(th.clip_grad_norm_([], 1.0)) == 0.0
+    new, n = th.clip_by_global_norm([], 1.0)
+    assert new == () and float(n) == 0.0 and float(th.global_norm([])) == 0.0
+    assert th.clip_grads_with_norm_([p], 1.0, torch.tensor(1.0)) is None
+
+
+def test_c_abi_refuses_bad_descriptors(lib):
+    good = dict(batch=1, channels=4, groups=2, nlat=8, nlon=16, dtype=0, param_dtype=0, channels_last=0, activation=0, eps=1e-5)
+    assert lib.shtb200_group_norm_workspace_bytes(_lib.GroupNormDesc(**good), 0) > 0
+    fake = 256  # never read: refused first
+    for bad in (dict(batch=-1), dict(channels=0), dict(groups=3), dict(groups=0), dict(nlat=0), dict(nlon=-4), dict(dtype=3), dict(dtype=-1), dict(param_dtype=7),
+                dict(activation=9), dict(eps=-1.0), dict(eps=math.nan), dict(batch=1 << 20, channels=1 << 10), dict(nlat=1 << 17, nlon=1 << 17)):  # fmt: skip
+        d = _lib.GroupNormDesc(**{**good, **bad})
+        assert lib.shtb200_group_norm_workspace_bytes(d, 0) == 0
+        assert lib.shtb200_group_norm_forward(d, fake, None, None, None, fake, fake, fake, 1 << 30, None) == -1
+        assert lib.shtb200_group_norm_backward(d, fake, fake, None, None, None, fake, fake, None, None, fake, 1 << 30, None) == -1
+    d = _lib.GroupNormDesc(**good)
+    assert lib.shtb200_group_norm_forward(None, fake, None, None, None, fake, fake, fake, 1 << 30, None) == -1
+    assert lib.shtb200_group_norm_forward(d, None, None, None, None, fake, fake, fake, 1 << 30, None) == -1
+    assert lib.shtb200_group_norm_forward(d, fake, None, None, None, fake, fake, fake, 8, None) == -3
+    assert lib.shtb200_group_norm_forward(d, fake, None, None, None, fake, fake, None, 1 << 30, None) == -3
+
+
+def _lists(tensors):
+    """(count, src, numel, dtype) from (address, entries, type) triples that are never read."""
+    n = len(tensors)
+    return n, (ctypes.c_uint64 * n)(*[t[0] for t in tensors]), (ctypes.c_int64 * n)(*[t[1] for t in tensors]), (ctypes.c_int32 * n)(*[t[2] for t in tensors])
+
+
+def test_c_abi_refuses_bad_tensor_lists(lib):
+    at = 1 << 20
+    ws, big = 1 << 16, 1 << 30
+
+    def clip(ts, dst=None, limit=1.0, kind=0, wsb=big):
+        n, src, numel, dtype = _lists(ts)
+        dst = src if dst is None else (ctypes.c_uint64 * n)(*dst)
+        return lib.shtb200_clip_grads(n, src, dst, numel, dtype, kind, limit, ws, ws, wsb, None)
+
+    assert clip([(at, 4, 0), (at + 8, 4, 0)]) == -1 and b"share memory" in lib.shtb200_last_error()
+    assert clip([(at, 4, 0), (at, 4, 0)]) == -1
+    assert clip([(at, 100, 3), (at + 16, 1, 1)]) == -1
+    assert clip([(at, 4, 0), (at + 64, 4, 0)], dst=[at + 64, at + 128]) == -1  # one's result on another's input
+    assert clip([(at, 4, 0)], dst=[at + 8]) == -1  # partly on its own input
+    assert clip([(at + 2, 4, 0)]) == -1 and b"aligned" in lib.shtb200_last_error()
+    assert clip([(at, -1, 0)]) == -1 and clip([(at, 4, 4)]) == -1 and clip([(0, 4, 0)]) == -1
+    assert clip([(at, 4, 0)], limit=-1.0) == -1 and clip([(at, 4, 0)], limit=math.nan) == -1 and clip([(at, 4, 0)], kind=5) == -1
+    assert clip([(at, 4, 0)], wsb=8) == -3
+    assert lib.shtb200_clip_grads(1, None, None, None, None, 0, 1.0, ws, ws, big, None) == -1
+    assert lib.shtb200_scale_grads(1, None, None, None, None, 1.0, ws, None) == -1
+
+
+def test_oracle_agrees_on_the_quadrature():
+    """The latitude weights are the oracle's too (independent formulas)."""
+    _, w = orc.colatitudes(13, "legendre-gauss")
+    m = th.GroupNormS2(1, 1, (13, 24), grid="legendre-gauss")
+    assert np.allclose(m.lat_weights.double().numpy(), w / np.mean(w), rtol=1e-6)

@@ -17,6 +17,18 @@ SHT, ISHT, SHT_ADJOINT, ISHT_ADJOINT, VSHT, IVSHT, VSHT_ADJOINT, IVSHT_ADJOINT =
 ENGINE_AUTO, ENGINE_SIMT, ENGINE_TCGEN05 = range(3)
 ENGINES = {"auto": ENGINE_AUTO, "simt": ENGINE_SIMT, "tcgen05": ENGINE_TCGEN05}
 
+# enum shtb200_dtype, shtb200_activation, shtb200_norm
+F32, BF16, F16, C64 = range(4)
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
+NORM_L2, NORM_INF = range(2)
+
+
+class GroupNormDesc(ctypes.Structure):
+    """struct shtb200_group_norm_desc"""
+
+    _fields_ = [(n, ctypes.c_int) for n in ("batch", "channels", "groups", "nlat", "nlon", "dtype", "param_dtype", "channels_last", "activation")] + [("eps", ctypes.c_float)]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -87,6 +99,20 @@ def load():
         lib.shtb200_spectral_conv.restype = ci
         lib.shtb200_quadrature.argtypes = [vp, vp, vp, cll, ci, ci, vp]
         lib.shtb200_quadrature.restype = ci
+        lib.shtb200_group_norm_workspace_bytes.argtypes = [ctypes.POINTER(GroupNormDesc), ci]
+        lib.shtb200_group_norm_workspace_bytes.restype = cs
+        lib.shtb200_group_norm_forward.argtypes = [ctypes.POINTER(GroupNormDesc)] + [vp] * 7 + [cs, vp]
+        lib.shtb200_group_norm_forward.restype = ci
+        lib.shtb200_group_norm_backward.argtypes = [ctypes.POINTER(GroupNormDesc)] + [vp] * 10 + [cs, vp]
+        lib.shtb200_group_norm_backward.restype = ci
+        lib.shtb200_grad_norm_workspace_bytes.argtypes = [ci]
+        lib.shtb200_grad_norm_workspace_bytes.restype = cs
+        lib.shtb200_grad_norm.argtypes = [ci, vp, vp, vp, ci, vp, vp, cs, vp]
+        lib.shtb200_grad_norm.restype = ci
+        lib.shtb200_clip_grads.argtypes = [ci, vp, vp, vp, vp, ci, ctypes.c_float, vp, vp, cs, vp]
+        lib.shtb200_clip_grads.restype = ci
+        lib.shtb200_scale_grads.argtypes = [ci, vp, vp, vp, vp, ctypes.c_float, vp, vp]
+        lib.shtb200_scale_grads.restype = ci
         _lib = lib
         return lib
 

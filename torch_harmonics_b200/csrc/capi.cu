@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <exception>
 #include <mutex>
 
 #include "common.cuh"
@@ -606,6 +607,55 @@ int shtb200_quadrature(const float *x_dev, const float *lat_weights_dev, float *
     if (nfields == 0) return SHTB200_OK;
     if (!x_dev || !lat_weights_dev || !out_dev) return fail(SHTB200_EINVAL, "null pointer");
     return launch_quadrature(x_dev, lat_weights_dev, out_dev, nfields, nlat, nlon, (cudaStream_t)stream);
+}
+
+// What is thrown on the way (an allocation of the host that fails) becomes an error code: nothing may pass a C entry point.
+#define SHT_GUARDED(expr)                                                          \
+    try {                                                                          \
+        return expr;                                                               \
+    } catch (const std::exception &e) {                                            \
+        try {                                                                      \
+            return fail(SHTB200_EINVAL, e.what());                                 \
+        } catch (...) {                                                            \
+            return SHTB200_EINVAL;                                                 \
+        }                                                                          \
+    }
+
+size_t shtb200_group_norm_workspace_bytes(const shtb200_group_norm_desc *desc, int backward) {
+    try {
+        return group_norm_workspace(desc, backward != 0);
+    } catch (const std::exception &) {
+        return 0;
+    }
+}
+
+int shtb200_group_norm_forward(const shtb200_group_norm_desc *desc, const void *x_dev, const float *lat_weights_dev, const void *weight_dev, const void *bias_dev, void *y_dev,
+                               void *stats_dev, void *workspace_dev, size_t workspace_bytes, void *stream) {
+    SHT_GUARDED(group_norm_forward(desc, x_dev, lat_weights_dev, weight_dev, bias_dev, y_dev, stats_dev, workspace_dev, workspace_bytes, (cudaStream_t)stream))
+}
+
+int shtb200_group_norm_backward(const shtb200_group_norm_desc *desc, const void *dy_dev, const void *x_dev, const float *lat_weights_dev, const void *weight_dev, const void *bias_dev,
+                                const void *stats_dev, void *dx_dev, void *dweight_dev, void *dbias_dev, void *workspace_dev, size_t workspace_bytes, void *stream) {
+    SHT_GUARDED(group_norm_backward(desc, dy_dev, x_dev, lat_weights_dev, weight_dev, bias_dev, stats_dev, dx_dev, dweight_dev, dbias_dev, workspace_dev, workspace_bytes,
+                                    (cudaStream_t)stream))
+}
+
+size_t shtb200_grad_norm_workspace_bytes(int count) { return grad_norm_workspace(count); }
+
+int shtb200_grad_norm(int count, const void *const *src_dev, const long long *numel, const int *dtype, int norm, float *norm_dev, void *workspace_dev, size_t workspace_bytes,
+                      void *stream) {
+    SHT_GUARDED(grad_norm(count, src_dev, numel, dtype, norm, norm_dev, workspace_dev, workspace_bytes, (cudaStream_t)stream))
+}
+
+int shtb200_clip_grads(int count, const void *const *src_dev, void *const *dst_dev, const long long *numel, const int *dtype, int norm, float max_norm, float *norm_dev,
+                       void *workspace_dev, size_t workspace_bytes, void *stream) {
+    if (count > 0 && !dst_dev) return fail(SHTB200_EINVAL, "null pointer");
+    SHT_GUARDED(clip_grads(count, src_dev, dst_dev, numel, dtype, norm, max_norm, norm_dev, workspace_dev, workspace_bytes, (cudaStream_t)stream))
+}
+
+int shtb200_scale_grads(int count, const void *const *src_dev, void *const *dst_dev, const long long *numel, const int *dtype, float max_norm, const float *norm_dev, void *stream) {
+    if (count > 0 && !dst_dev) return fail(SHTB200_EINVAL, "null pointer");
+    SHT_GUARDED(scale_grads(count, src_dev, dst_dev, numel, dtype, max_norm, norm_dev, (cudaStream_t)stream))
 }
 
 int shtb200_plan_info(const shtb200_plan *pl, int *nlat, int *nlon, int *lmax, int *mmax, int *kind, int *engine) {

@@ -268,6 +268,19 @@ size_t slab_mix_weight_bytes(int cin, int cout, int ngroups, int lmax);
 int launch_slab_mix(const Plan &pl, const float *Zin, float *Zout, const float2 *weight, float2 *wsplit, int batch, int cin, int cout, int ngroups, cudaStream_t st);
 int launch_quadrature(const float *x, const float *w, float *out, long long nfields, int nlat, int nlon, cudaStream_t st);
 
+// group normalisation with an activation (group_norm.cu), gradient norm and clipping (grad_norm.cu)
+using GroupNormDesc = ::shtb200_group_norm_desc;
+size_t group_norm_workspace(const GroupNormDesc *d, bool backward);
+int group_norm_forward(const GroupNormDesc *d, const void *x, const float *lat, const void *weight, const void *bias, void *y, void *stats, void *ws, size_t ws_bytes,
+                       cudaStream_t st);
+int group_norm_backward(const GroupNormDesc *d, const void *dy, const void *x, const float *lat, const void *weight, const void *bias, const void *stats, void *dx, void *dweight,
+                        void *dbias, void *ws, size_t ws_bytes, cudaStream_t st);
+size_t grad_norm_workspace(int count);
+int grad_norm(int count, const void *const *src, const long long *numel, const int *dtype, int kind, float *norm, void *ws, size_t ws_bytes, cudaStream_t st);
+int scale_grads(int count, const void *const *src, void *const *dst, const long long *numel, const int *dtype, float max_norm, const float *norm, cudaStream_t st);
+int clip_grads(int count, const void *const *src, void *const *dst, const long long *numel, const int *dtype, int kind, float max_norm, float *norm, void *ws, size_t ws_bytes,
+               cudaStream_t st);
+
 // Row of (group, k) in the column-contiguous operands X and Y: 32-row blocks of k are outermost, then the group,
 // then k inside the block.  CTAs of the FFT kernels that run at the same time work on neighbouring k for ALL groups,
 // so with this order they fill / read one contiguous region of HBM instead of 2 * mmax far-apart ones, and the

@@ -1,0 +1,186 @@
+"""The global norm of a set of gradients, and clipping to a largest norm, for training the layers of this package: float32,
+bfloat16, float16 and complex64 gradients (the weights of ``SpectralConvS2``) together, in two launches whatever their number.
+
+``clip_grad_norm_`` is used like ``torch.nn.utils.clip_grad_norm_``.  Sums of squares are float64, the norm is a float32 scalar on the
+gradients' device, and nothing waits for the device.  Where the norm is within the limit the gradients are not touched.
+
+Where parameters are sharded over processes (``distributed.DistributedSpectralConvS2`` keeps its own degrees on each rank), take
+``global_norm`` of the sharded and of the replicated gradients on every rank, add the squares of the former over the group,
+and hand the joined norm to ``clip_grads_with_norm_``.
+"""
+
+import math
+from array import array
+from typing import Iterable, Tuple, Union
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.complex64: _lib.C64}
+
+
+def _norm_kind(norm_type):
+    norm_type = float(norm_type)
+    if norm_type == 2.0:
+        return _lib.NORM_L2
+    if norm_type == math.inf:
+        return _lib.NORM_INF
+    raise ValueError(f"norm_type must be 2 or inf, got {norm_type}")
+
+
+def _limit(max_norm):
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must be non-negative, got {max_norm}")
+    return max_norm
+
+
+def _fills_memory(t):
+    """Whether the entries of ``t`` are a gapless stretch of memory, in any order of the axes."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for stride, size in sorted(zip(t.stride(), t.shape)):
+        if size != 1:
+            if stride != expect:
+                return False
+            expect *= size
+    return True
+
+
+def _check(tensors, what):
+    for t in tensors:
+        if not t.is_cuda:
+            raise RuntimeError(f"{what}: expected CUDA tensors; torch_harmonics_b200 has no CPU path")
+        if t.layout != torch.strided:
+            raise TypeError(f"{what}: expected dense tensors, got {t.layout}")
+        if t.dtype not in _DTYPES:
+            raise TypeError(f"{what}: expected float32, bfloat16, float16 or complex64 tensors, got {t.dtype}")
+        if t.device != tensors[0].device:
+            raise RuntimeError(f"{what}: all tensors must be on one device, got {tensors[0].device} and {t.device}")
+
+
+class _List:
+    """The tensors of a call as host arrays for the C ABI."""
+
+    def __init__(self, tensors):
+        self.n = len(tensors)
+        self._src = array("Q", [t.data_ptr() for t in tensors])
+        self._numel = array("q", [t.numel() for t in tensors])
+        self._dtype = array("i", [_DTYPES[t.dtype] for t in tensors])
+        self.src, self.numel, self.dtype = (a.buffer_info()[0] for a in (self._src, self._numel, self._dtype))
+
+
+def _norm(tensors, kind):
+    dev = tensors[0].device
+    lib, ls = _lib.load(), _List(tensors)
+    nbytes = lib.shtb200_grad_norm_workspace_bytes(ls.n)
+    ws, norm = torch.empty(nbytes, dtype=torch.uint8, device=dev), torch.empty((), dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        rc = lib.shtb200_grad_norm(ls.n, ls.src, ls.numel, ls.dtype, kind, norm.data_ptr(), ws.data_ptr(), nbytes, torch.cuda.current_stream(dev).cuda_stream)
+    _lib.check(rc, "shtb200_grad_norm")
+    return norm
+
+
+def _clip(src, dst, max_norm, kind, norm=None):
+    """dst = src clipped; returns the norm, which is computed unless it is given."""
+    dev = src[0].device
+    lib, ls = _lib.load(), _List(src)
+    to = ls._src if dst is src else array("Q", [t.data_ptr() for t in dst])
+    with torch.cuda.device(dev):
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        if norm is not None:
+            rc = lib.shtb200_scale_grads(ls.n, ls.src, to.buffer_info()[0], ls.numel, ls.dtype, max_norm, norm.data_ptr(), stream)
+        else:
+            nbytes = lib.shtb200_grad_norm_workspace_bytes(ls.n)
+            ws, norm = torch.empty(nbytes, dtype=torch.uint8, device=dev), torch.empty((), dtype=torch.float32, device=dev)
+            rc = lib.shtb200_clip_grads(ls.n, ls.src, to.buffer_info()[0], ls.numel, ls.dtype, kind, max_norm, norm.data_ptr(), ws.data_ptr(), nbytes, stream)
+    _lib.check(rc, "shtb200_clip_grads")
+    return norm
+
+
+def _refuse_nonfinite(norm, norm_type):
+    if not math.isfinite(norm.item()):
+        raise RuntimeError(f"The total norm of order {float(norm_type)} of the gradients is non-finite, so it cannot be clipped.")
+
+
+def _grads(parameters, what):
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    grads = [p.grad for p in parameters if p.grad is not None]
+    _check(grads, what)
+    return grads
+
+
+def _clip_in_place(grads, max_norm, kind, norm=None):
+    held = [g if _fills_memory(g) else g.contiguous() for g in grads]  # (a slice of a larger tensor is clipped in a copy)
+    norm = _clip(held, held, max_norm, kind, norm)
+    for g, h in zip(grads, held):
+        if h is not g:
+            g.copy_(h)
+    torch.autograd.graph.increment_version(grads)
+    return norm
+
+
+@torch.no_grad()
+def global_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0) -> torch.Tensor:
+    """The norm of all entries of ``tensors`` together (``norm_type`` 2 or inf), a float32 scalar; zero for no tensors."""
+    kind = _norm_kind(norm_type)
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    _check(tensors, "global_norm")
+    if not tensors:
+        return torch.tensor(0.0)
+    return _norm([t if _fills_memory(t) else t.contiguous() for t in tensors], kind)
+
+
+@torch.no_grad()
+def clip_grad_norm_(
+    parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False
+) -> torch.Tensor:
+    """Scale the gradients of ``parameters`` in place by ``min(1, max_norm / (norm + 1e-6))`` and return the norm they had.
+
+    Parameters without a gradient are left out; gradients that share memory are refused.  A norm that is not finite makes the gradients zero or NaN, or
+    raises with ``error_if_nonfinite`` (which waits for the device), before any gradient is touched."""
+    kind, max_norm = _norm_kind(norm_type), _limit(max_norm)
+    grads = _grads(parameters, "clip_grad_norm_")
+    if not grads:
+        return torch.tensor(0.0)
+    norm = None
+    if error_if_nonfinite:
+        norm = global_norm(grads, norm_type)
+        _refuse_nonfinite(norm, norm_type)
+    return _clip_in_place(grads, max_norm, kind, norm)
+
+
+@torch.no_grad()
+def clip_grads_with_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, total_norm: torch.Tensor) -> None:
+    """``clip_grad_norm_`` with a norm that is known: a scalar on the gradients' device, e.g. one joined over several processes."""
+    max_norm = _limit(max_norm)
+    grads = _grads(parameters, "clip_grads_with_norm_")
+    if not grads:
+        return
+    if total_norm.numel() != 1 or total_norm.device != grads[0].device:
+        raise RuntimeError(f"clip_grads_with_norm_: expected total_norm as a scalar on {grads[0].device}, got shape {tuple(total_norm.shape)} on {total_norm.device}")
+    _clip_in_place(grads, max_norm, _lib.NORM_L2, total_norm.to(torch.float32).contiguous())
+
+
+@torch.no_grad()
+def clip_by_global_norm(
+    tensors: Iterable[torch.Tensor], max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False
+) -> Tuple[Tuple[torch.Tensor, ...], torch.Tensor]:
+    """``(clipped, norm)``: new tensors ``min(1, max_norm / (norm + 1e-6)) * t`` and the norm of ``tensors``, which stay as they are
+    (the gradients that ``torch.autograd.grad`` returns, or those of one micro-batch before they are accumulated)."""
+    kind, max_norm = _norm_kind(norm_type), _limit(max_norm)
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    _check(tensors, "clip_by_global_norm")
+    if not tensors:
+        return (), torch.tensor(0.0)
+    src = [t.resolve_conj().resolve_neg() if _fills_memory(t) else _lib.dense(t) for t in tensors]
+    norm = None
+    if error_if_nonfinite:
+        norm = _norm(src, kind)
+        _refuse_nonfinite(norm, norm_type)
+    dst = [torch.empty_like(t) for t in src]
+    norm = _clip(src, dst, max_norm, kind, norm)
+    return tuple(dst), norm

@@ -1,0 +1,190 @@
+"""Group normalisation on the sphere, fused with the activation behind it.
+
+The mean and variance of a group are those of a field on the sphere: averages over its channels and grid points with the
+latitude quadrature weights of the grid (``QuadratureS2``), so that the many grid points near the poles do not count for more than
+their area.  ``weighted=False`` gives the plain averages over grid points of ordinary group normalisation.
+"""
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .quadrature import precompute_latitudes, trapezoidal_weights
+
+_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _latitude_weights(nlat, grid):
+    if grid == "equiangular-trapezoidal":
+        return trapezoidal_weights(nlat, -1, 1)[1]
+    return precompute_latitudes(nlat, grid)[1]
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _run(module, x, weight, bias):
+    """y and what the backward pass needs, for a dense ``x``."""
+    desc, nbytes, _ = module._call(x)
+    y = torch.empty_like(x)
+    stats = torch.empty(x.shape[0], module.num_groups, 4, dtype=torch.float32, device=x.device)
+    if x.shape[0] == 0:
+        return y, stats
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+        rc = _lib.load().shtb200_group_norm_forward(
+            desc, x.data_ptr(), _ptr(module.lat_weights), _ptr(weight), _ptr(bias), y.data_ptr(), stats.data_ptr(), ws.data_ptr(), nbytes, torch.cuda.current_stream(x.device).cuda_stream
+        )
+    _lib.check(rc, "shtb200_group_norm_forward")
+    return y, stats
+
+
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, module):
+        y, stats = _run(module, x, weight, bias)
+        ctx.save_for_backward(x, weight, bias, stats, module.lat_weights)
+        ctx.call = module._call(x)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, stats, lat = ctx.saved_tensors
+        desc, _, nbytes = ctx.call
+        dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
+        dw = torch.zeros_like(weight) if ctx.needs_input_grad[1] else None
+        db = torch.zeros_like(bias) if ctx.needs_input_grad[2] else None
+        if x.shape[0] == 0:
+            return dx, dw, db, None
+        # the gradient comes in any layout (an expanded scalar, for a sum): the kernel reads it in the layout of x
+        dy = _lib.dense(dy) if not desc.channels_last else dy.resolve_neg().contiguous(memory_format=torch.channels_last)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        with torch.cuda.device(x.device):
+            rc = _lib.load().shtb200_group_norm_backward(
+                desc, dy.data_ptr(), x.data_ptr(), _ptr(lat), _ptr(weight), _ptr(bias), stats.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(), nbytes,
+                torch.cuda.current_stream(x.device).cuda_stream,
+            )
+        _lib.check(rc, "shtb200_group_norm_backward")
+        return dx, dw, db, None
+
+
+class GroupNormS2(nn.Module):
+    """``(batch, num_channels, nlat, nlon) -> `` the same shape: normalise each of ``num_groups`` groups of consecutive channels
+    by its mean and variance over the sphere, scale and shift every channel (``weight``, ``bias``), apply ``activation``.
+
+    ``num_groups = num_channels`` is instance normalisation, ``num_groups = 1`` layer normalisation over (channels, sphere).
+
+    Parameters
+    ----------
+    img_shape : (nlat, nlon)
+    grid : the latitude grid whose quadrature weights are used: "equiangular", "legendre-gauss", "lobatto" or "equiangular-trapezoidal"
+    eps : added to the variance
+    affine : whether ``weight`` and ``bias`` (num_channels,) exist
+    activation : None, "relu", "silu" or "gelu" (z times the normal distribution function, exact form)
+    weighted : False: every grid point counts the same, whatever the grid
+
+    The input is float32, bfloat16 or float16, in planes (contiguous) or channels last (``torch.channels_last``); both are read
+    where they are, other strides are copied first.  The output has the input's type and layout; statistics, sums and the
+    activation are float32 or wider whatever the type, under autocast too.  The parameters may have any of the three types.  The
+    gradients can be computed once (no second derivatives).
+    """
+
+    def __init__(
+        self,
+        num_groups: int,
+        num_channels: int,
+        img_shape: Tuple[int],
+        grid: Optional[str] = "equiangular",
+        eps: Optional[float] = 1e-5,
+        affine: Optional[bool] = True,
+        activation: Optional[str] = None,
+        weighted: Optional[bool] = True,
+    ):
+        super().__init__()
+        if num_groups < 1 or num_channels < 1:
+            raise ValueError(f"num_groups ({num_groups}) and num_channels ({num_channels}) must be positive")
+        if num_channels % num_groups != 0:
+            raise ValueError(f"num_channels ({num_channels}) must be divisible by num_groups ({num_groups})")
+        if activation not in _lib.ACTIVATIONS:
+            raise ValueError(f"Unknown activation {activation!r}, expected one of {list(_lib.ACTIVATIONS)}")
+        if not eps >= 0.0:
+            raise ValueError(f"eps must be non-negative, got {eps}")
+        self.num_groups = num_groups
+        self.num_channels = num_channels
+        self.nlat, self.nlon = img_shape
+        self.grid = grid
+        self.eps = eps
+        self.activation = activation
+        self.weighted = weighted
+        if affine:
+            self.weight = nn.Parameter(torch.ones(num_channels))
+            self.bias = nn.Parameter(torch.zeros(num_channels))
+        else:
+            self.register_parameter("weight", None)
+            self.register_parameter("bias", None)
+        lat = None
+        if weighted:
+            lat = _latitude_weights(self.nlat, grid)
+            lat = (lat / lat.mean()).to(torch.float32)
+        self.register_buffer("lat_weights", lat, persistent=False)
+        self._calls = {}
+
+    def extra_repr(self):
+        return f"num_groups={self.num_groups}, num_channels={self.num_channels}, nlat={self.nlat}, nlon={self.nlon},\n grid={self.grid}, eps={self.eps}, activation={self.activation}, weighted={self.weighted}"
+
+    def _apply(self, fn, *args, **kwargs):
+        # the module may be cast to half precision: the latitude weights move with it but stay float32
+        lat = self.lat_weights
+        out = super()._apply(fn, *args, **kwargs)
+        if lat is not None and self.lat_weights.dtype != lat.dtype:
+            self.lat_weights = lat.to(device=self.lat_weights.device)
+        return out
+
+    def __getstate__(self):
+        state = super().__getstate__() if hasattr(super(), "__getstate__") else self.__dict__
+        return {**state, "_calls": {}}
+
+    def _call(self, x):
+        """(descriptor, workspace bytes forward, backward) of a call on ``x``: shapes and types only."""
+        param = torch.float32 if self.weight is None else self.weight.dtype
+        cl = not x.is_contiguous()
+        key = (x.shape[0], x.dtype, param, cl, self.eps, self.activation)
+        call = self._calls.get(key)
+        if call is None:
+            desc = _lib.GroupNormDesc(
+                x.shape[0], self.num_channels, self.num_groups, self.nlat, self.nlon, _DTYPES[x.dtype], _DTYPES[param], int(cl), _lib.ACTIVATIONS[self.activation], self.eps
+            )
+            ws = [_lib.load().shtb200_group_norm_workspace_bytes(desc, i) for i in (0, 1)]
+            if ws[0] == 0:
+                _lib.check(-1, "shtb200_group_norm_workspace_bytes")
+            call = self._calls[key] = (desc, *ws)
+        return call
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if not x.is_cuda:
+            raise RuntimeError("GroupNormS2: expected a CUDA tensor; torch_harmonics_b200 has no CPU path")
+        if x.dtype not in _DTYPES:
+            raise TypeError(f"GroupNormS2: expected dtype torch.float32, torch.bfloat16 or torch.float16, got {x.dtype}")
+        if x.dim() != 4:
+            raise RuntimeError(f"Expected tensor with 4 dimensions but got {x.dim()} instead")
+        if x.shape[1:] != (self.num_channels, self.nlat, self.nlon):
+            raise RuntimeError(f"Expected shape (batch, {self.num_channels}, {self.nlat}, {self.nlon}), got {tuple(x.shape)}")
+        weight, bias = self.weight, self.bias
+        if weight is not None:
+            if weight.device != x.device or bias.device != x.device:
+                raise RuntimeError(f"GroupNormS2: the input is on {x.device}, the parameters on {weight.device}")
+            if weight.dtype not in _DTYPES or bias.dtype != weight.dtype:
+                raise TypeError(f"GroupNormS2: weight and bias must both be float32, bfloat16 or float16, got {weight.dtype} and {bias.dtype}")
+        elif self.lat_weights is not None and self.lat_weights.device != x.device:
+            raise RuntimeError(f"GroupNormS2: the input is on {x.device}, the latitude weights on {self.lat_weights.device}")
+        if not (x.is_contiguous() or x.is_contiguous(memory_format=torch.channels_last)) or x.is_neg():
+            x = _lib.dense(x)
+        if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and (weight.requires_grad or bias.requires_grad))):
+            return _GroupNorm.apply(x, weight, bias, self)
+        return _run(self, x, weight, bias)[0]
