@@ -21,8 +21,11 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTensors = 896;         // tensors of one launch: the table has to fit into 32,764 bytes of kernel arguments
-constexpr int kChunk = 8192;             // values of one unit of work
-constexpr int kMaxBlocks = 148 * 4;
+constexpr int kUnitBytes = 32768;        // one unit of work: 8 vectors of 16 bytes a thread, all of them in flight before the first is used
+constexpr int kVectors = kUnitBytes / 16 / kThreads;
+constexpr int kScaleVectors = 4;         // (eight in flight spill: the scaling kernel also holds the addresses it writes to)
+constexpr int kBlocksPerSm = 4;
+constexpr int kMaxBlocks = 148 * kBlocksPerSm;
 
 struct Table {
     const void *src[kMaxTensors];
@@ -34,19 +37,47 @@ struct Table {
 };
 static_assert(sizeof(Table) + 64 <= 32764, "kernel arguments");
 
-__device__ __forceinline__ float load_value(const void *p, int dtype, long long i) {
-    if (dtype == SHTB200_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[i]);
-    if (dtype == SHTB200_F16) return __half2float(reinterpret_cast<const __half *>(p)[i]);
-    return reinterpret_cast<const float *>(p)[i];
+__host__ __device__ constexpr int unit_values(int dtype) { return dtype == SHTB200_BF16 || dtype == SHTB200_F16 ? kUnitBytes / 2 : kUnitBytes / 4; }
+
+template <typename T> struct Pack {  // 16 bytes of values
+    static constexpr int n = 16 / sizeof(T);
+    uint4 v;
+    __device__ __forceinline__ float get(int i) const;
+    __device__ __forceinline__ void scale(float f);
+};
+template <> __device__ __forceinline__ float Pack<float>::get(int i) const { return __uint_as_float(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w); }
+template <> __device__ __forceinline__ float Pack<__nv_bfloat16>::get(int i) const {
+    const unsigned u = i < 2 ? v.x : i < 4 ? v.y : i < 6 ? v.z : v.w;
+    return __uint_as_float(i & 1 ? u & 0xffff0000u : u << 16);
 }
-__device__ __forceinline__ void store_value(void *p, int dtype, long long i, float v) {
-    if (dtype == SHTB200_BF16) reinterpret_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
-    else if (dtype == SHTB200_F16) reinterpret_cast<__half *>(p)[i] = __float2half_rn(v);
-    else reinterpret_cast<float *>(p)[i] = v;
+template <> __device__ __forceinline__ float Pack<__half>::get(int i) const {
+    const unsigned u = i < 2 ? v.x : i < 4 ? v.y : i < 6 ? v.z : v.w;
+    return __half2float(__ushort_as_half((unsigned short)(i & 1 ? u >> 16 : u & 0xffffu)));
+}
+__device__ __forceinline__ float load_one(const float *p) { return *p; }
+__device__ __forceinline__ float load_one(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float load_one(const __half *p) { return __half2float(*p); }
+__device__ __forceinline__ void store_one(float *p, float v) { *p = v; }
+__device__ __forceinline__ void store_one(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void store_one(__half *p, float v) { *p = __float2half_rn(v); }
+template <> __device__ __forceinline__ void Pack<float>::scale(float f) {
+    v = make_uint4(__float_as_uint(get(0) * f), __float_as_uint(get(1) * f), __float_as_uint(get(2) * f), __float_as_uint(get(3) * f));
+}
+template <> __device__ __forceinline__ void Pack<__nv_bfloat16>::scale(float f) {
+    __nv_bfloat162 r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __floats2bfloat162_rn(get(2 * i) * f, get(2 * i + 1) * f);
+    v = *reinterpret_cast<uint4 *>(r);
+}
+template <> __device__ __forceinline__ void Pack<__half>::scale(float f) {
+    __half2 r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __floats2half2_rn(get(2 * i) * f, get(2 * i + 1) * f);
+    v = *reinterpret_cast<uint4 *>(r);
 }
 
-__device__ __forceinline__ int tensor_of(const Table &t, int unit) {
-    int lo = 0, hi = t.count;
+// Last tensor that starts at or before `unit`, searched from `lo` on (the units of a block ascend or descend).
+__device__ __forceinline__ int tensor_of(const Table &t, int unit, int lo, int hi) {
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (t.first[mid] <= unit) lo = mid;
@@ -58,7 +89,7 @@ __device__ __forceinline__ int tensor_of(const Table &t, int unit) {
 // (fmax drops a NaN; the largest magnitude has to keep it)
 __device__ __forceinline__ double larger(double a, double b) { return (b > a || b != b) ? b : a; }
 
-__device__ double block_join(double v, int kind) {
+template <int kind> __device__ double block_join(double v) {
     __shared__ double s[kThreads / 32];
     for (int o = 16; o; o >>= 1) {
         const double u = __shfl_xor_sync(0xffffffffu, v, o);
@@ -72,45 +103,112 @@ __device__ double block_join(double v, int kind) {
     return t;
 }
 
-// partial sums of squares (or largest squared magnitudes): one float64 value a block
-__global__ void __launch_bounds__(kThreads) norm_partial_kernel(const __grid_constant__ Table t, int kind, double *part) {
-    double acc = 0.;
-    const int units = t.first[t.count];
-    for (int u = blockIdx.x; u < units; u += gridDim.x) {
-        const int k = tensor_of(t, u);
-        const long long lo = (long long)(u - t.first[k]) * kChunk, hi = min(lo + kChunk, t.n[k]);
-        const int dt = t.dtype[k];
-        if (kind == SHTB200_NORM_INF && dt == SHTB200_C64) {
-            for (long long i = lo + 2 * threadIdx.x; i < hi; i += 2 * kThreads) {
-                const double re = load_value(t.src[k], dt, i), im = load_value(t.src[k], dt, i + 1);
-                acc = larger(acc, re * re + im * im);
-            }
-        } else {
-            for (long long i = lo + threadIdx.x; i < hi; i += kThreads) {
-                const double v = load_value(t.src[k], dt, i);
-                acc = kind == SHTB200_NORM_INF ? larger(acc, v * v) : fma(v, v, acc);
-            }
+// The squares are added in float64: their range (1e-45^2 to 3e38^2) is float64's, and no sum of any length loses anything.
+// pairs: entries are complex, their magnitude joins two values (for the largest magnitude; a sum of squares need not know).
+template <int kind, typename T>
+__device__ __forceinline__ void gather_unit(const T *p, int n, bool pairs, double acc[2]) {
+    const int head = min(n, (int)((16 - ((uintptr_t)p & 15)) & 15) / (int)sizeof(T));
+    if (kind == SHTB200_NORM_INF && pairs) {  // float pairs, 8-byte aligned: vector or not, a pair is never split
+        for (int i = 2 * threadIdx.x; i < n; i += 2 * kThreads) {
+            const double re = load_one(p + i), im = load_one(p + i + 1);
+            acc[0] = larger(acc[0], fma(re, re, im * im));
         }
+        return;
     }
-    acc = block_join(acc, kind);
-    if (threadIdx.x == 0) part[blockIdx.x] = acc;
+    const uint4 *q = reinterpret_cast<const uint4 *>(p + head);
+    const int vecs = (n - head) / Pack<T>::n;
+    Pack<T> v[kVectors];
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k) {
+        const int i = threadIdx.x + k * kThreads;
+        v[k].v = i < vecs ? __ldg(q + i) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k)
+#pragma unroll
+        for (int i = 0; i < Pack<T>::n; ++i) {
+            const double x = v[k].get(i);
+            acc[i & 1] = kind == SHTB200_NORM_INF ? larger(acc[i & 1], fabs(x)) : fma(x, x, acc[i & 1]);
+        }
+    const int rest = n - vecs * Pack<T>::n;  // values before and behind the vectors: fewer than 2 Pack::n
+    if ((int)threadIdx.x < rest) {
+        const double x = load_one(p + ((int)threadIdx.x < head ? threadIdx.x : vecs * Pack<T>::n + threadIdx.x));
+        acc[0] = kind == SHTB200_NORM_INF ? larger(acc[0], fabs(x)) : fma(x, x, acc[0]);
+    }
 }
 
-__device__ float total_norm(const double *part, int nparts, int kind) {
+// Partial sums of squares (or largest magnitudes, squared): one float64 value a block.
+template <int kind>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) norm_partial_kernel(const __grid_constant__ Table t, double *part) {
+    double acc[2] = {0., 0.}, pair[2] = {0., 0.};
+    const int units = t.first[t.count];
+    int k = 0;
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+        k = tensor_of(t, u, k, t.count);
+        const int dt = t.dtype[k], uv = unit_values(dt);
+        const long long lo = (long long)(u - t.first[k]) * uv;
+        const int n = (int)min((long long)uv, t.n[k] - lo);
+        if (dt == SHTB200_BF16) gather_unit<kind>(reinterpret_cast<const __nv_bfloat16 *>(t.src[k]) + lo, n, false, acc);
+        else if (dt == SHTB200_F16) gather_unit<kind>(reinterpret_cast<const __half *>(t.src[k]) + lo, n, false, acc);
+        else if (kind == SHTB200_NORM_INF && dt == SHTB200_C64) gather_unit<kind>(reinterpret_cast<const float *>(t.src[k]) + lo, n, true, pair);
+        else gather_unit<kind>(reinterpret_cast<const float *>(t.src[k]) + lo, n, false, acc);
+    }
+    double v = kind == SHTB200_NORM_INF ? larger(acc[0], acc[1]) : acc[0] + acc[1];
+    if (kind == SHTB200_NORM_INF) v = larger(v * v, pair[0]);
+    v = block_join<kind>(v);
+    if (threadIdx.x == 0) part[blockIdx.x] = v;
+}
+
+template <int kind> __device__ float total_norm(const double *part, int nparts) {
     double acc = 0.;
     for (int i = threadIdx.x; i < nparts; i += kThreads) acc = kind == SHTB200_NORM_INF ? larger(acc, part[i]) : acc + part[i];
-    return (float)sqrt(block_join(acc, kind));
+    return (float)sqrt(block_join<kind>(acc));
 }
 
-__global__ void __launch_bounds__(kThreads) norm_total_kernel(const double *part, int nparts, int kind, float *norm) {
-    const float v = total_norm(part, nparts, kind);
+template <int kind>
+__global__ void __launch_bounds__(kThreads) norm_total_kernel(const double *part, int nparts, float *norm) {
+    const float v = total_norm<kind>(part, nparts);
     if (threadIdx.x == 0) *norm = v;
 }
 
-__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ Table t, const double *part, int nparts, int kind, float max_norm, float *norm) {
+template <typename T>
+__device__ __forceinline__ void scale_unit(const T *p, T *d, int n, float f) {
+    if ((((uintptr_t)p ^ (uintptr_t)d) & 15) != 0) {  // no vector is aligned on both sides
+        for (int i = threadIdx.x; i < n; i += kThreads) store_one(d + i, load_one(p + i) * f);
+        return;
+    }
+    const int head = min(n, (int)((16 - ((uintptr_t)p & 15)) & 15) / (int)sizeof(T));
+    const uint4 *q = reinterpret_cast<const uint4 *>(p + head);
+    uint4 *o = reinterpret_cast<uint4 *>(d + head);
+    const int vecs = (n - head) / Pack<T>::n;
+#pragma unroll 1
+    for (int r = 0; r < kVectors; r += kScaleVectors) {
+        Pack<T> v[kScaleVectors];
+#pragma unroll
+        for (int k = 0; k < kScaleVectors; ++k) {
+            const int i = threadIdx.x + (r + k) * kThreads;
+            v[k].v = i < vecs ? q[i] : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < kScaleVectors; ++k) {
+            const int i = threadIdx.x + (r + k) * kThreads;
+            v[k].scale(f);
+            if (i < vecs) o[i] = v[k].v;
+        }
+    }
+    const int rest = n - vecs * Pack<T>::n;
+    if ((int)threadIdx.x < rest) {
+        const int i = (int)threadIdx.x < head ? threadIdx.x : vecs * Pack<T>::n + threadIdx.x;
+        store_one(d + i, load_one(p + i) * f);
+    }
+}
+
+// The units are taken from the end: what the norm has read last is still in L2.
+template <int kind>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) scale_kernel(const __grid_constant__ Table t, const double *part, int nparts, float max_norm, float *norm) {
     float total;
     if (part) {
-        total = total_norm(part, nparts, kind);
+        total = total_norm<kind>(part, nparts);
         if (blockIdx.x == 0 && threadIdx.x == 0) *norm = total;
     } else {
         total = *norm;
@@ -118,12 +216,16 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__
     float f = max_norm / (total + 1e-6f);
     if (f > 1.f) f = 1.f;  // (a NaN stays one)
     const int units = t.first[t.count];
-    for (int u = blockIdx.x; u < units; u += gridDim.x) {
-        const int k = tensor_of(t, u);
+    int k = t.count - 1;
+    for (int u = units - 1 - (int)blockIdx.x; u >= 0; u -= gridDim.x) {
+        k = tensor_of(t, u, 0, k + 1);
         if (f == 1.f && t.dst[k] == t.src[k]) continue;
-        const long long lo = (long long)(u - t.first[k]) * kChunk, hi = min(lo + kChunk, t.n[k]);
-        const int dt = t.dtype[k];
-        for (long long i = lo + threadIdx.x; i < hi; i += kThreads) store_value(t.dst[k], dt, i, load_value(t.src[k], dt, i) * f);
+        const int dt = t.dtype[k], uv = unit_values(dt);
+        const long long lo = (long long)(u - t.first[k]) * uv;
+        const int n = (int)min((long long)uv, t.n[k] - lo);
+        if (dt == SHTB200_BF16) scale_unit(reinterpret_cast<const __nv_bfloat16 *>(t.src[k]) + lo, reinterpret_cast<__nv_bfloat16 *>(t.dst[k]) + lo, n, f);
+        else if (dt == SHTB200_F16) scale_unit(reinterpret_cast<const __half *>(t.src[k]) + lo, reinterpret_cast<__half *>(t.dst[k]) + lo, n, f);
+        else scale_unit(reinterpret_cast<const float *>(t.src[k]) + lo, reinterpret_cast<float *>(t.dst[k]) + lo, n, f);
     }
 }
 
@@ -171,7 +273,7 @@ std::vector<Table> make_tables(int count, const void *const *src, void *const *d
     long long units = 0;
     for (int i = 0; i < count; ++i) {
         if (numel[i] == 0) continue;
-        const long long n = numel[i] * (dtype[i] == SHTB200_C64 ? 2 : 1), u = (n + kChunk - 1) / kChunk;
+        const long long n = numel[i] * (dtype[i] == SHTB200_C64 ? 2 : 1), u = (n + unit_values(dtype[i]) - 1) / unit_values(dtype[i]);
         if (tables.empty() || tables.back().count == kMaxTensors) {
             tables.emplace_back();
             units = 0;
@@ -194,10 +296,14 @@ int blocks_of(const Table &t) { return std::min(kMaxBlocks, t.first[t.count]); }
 int launch_partials(const std::vector<Table> &tables, int kind, double *part, cudaStream_t st) {
     int nparts = 0;
     for (const Table &t : tables) {
-        norm_partial_kernel<<<blocks_of(t), kThreads, 0, st>>>(t, kind, part + nparts);
+        (kind == SHTB200_NORM_INF ? norm_partial_kernel<SHTB200_NORM_INF> : norm_partial_kernel<SHTB200_NORM_L2>)<<<blocks_of(t), kThreads, 0, st>>>(t, part + nparts);
         nparts += blocks_of(t);
     }
     return nparts;
+}
+
+void launch_total(const double *part, int nparts, int kind, float *norm, cudaStream_t st) {
+    (kind == SHTB200_NORM_INF ? norm_total_kernel<SHTB200_NORM_INF> : norm_total_kernel<SHTB200_NORM_L2>)<<<1, kThreads, 0, st>>>(part, nparts, norm);
 }
 
 int check_norm(int count, int kind, const float *norm, const void *ws, size_t ws_bytes) {
@@ -216,7 +322,7 @@ int grad_norm(int count, const void *const *src, const long long *numel, const i
     const std::vector<Table> tables = make_tables(count, src, nullptr, numel, dtype);
     double *part = reinterpret_cast<double *>(ws);
     const int nparts = launch_partials(tables, kind, part, st);
-    norm_total_kernel<<<1, kThreads, 0, st>>>(part, nparts, kind, norm);
+    launch_total(part, nparts, kind, norm, st);
     SHT_CUDA_CHECK(cudaGetLastError());
     return SHTB200_OK;
 }
@@ -229,8 +335,9 @@ int clip_grads(int count, const void *const *src, void *const *dst, const long l
     const std::vector<Table> tables = make_tables(count, src, dst, numel, dtype);
     double *part = reinterpret_cast<double *>(ws);
     const int nparts = launch_partials(tables, kind, part, st);
-    if (tables.empty()) norm_total_kernel<<<1, kThreads, 0, st>>>(part, nparts, kind, norm);
-    for (const Table &t : tables) scale_kernel<<<blocks_of(t), kThreads, 0, st>>>(t, part, nparts, kind, max_norm, norm);
+    if (tables.empty()) launch_total(part, nparts, kind, norm, st);
+    for (const Table &t : tables)
+        (kind == SHTB200_NORM_INF ? scale_kernel<SHTB200_NORM_INF> : scale_kernel<SHTB200_NORM_L2>)<<<blocks_of(t), kThreads, 0, st>>>(t, part, nparts, max_norm, norm);
     SHT_CUDA_CHECK(cudaGetLastError());
     return SHTB200_OK;
 }
@@ -240,7 +347,7 @@ int scale_grads(int count, const void *const *src, void *const *dst, const long 
     if (!norm) return fail(SHTB200_EINVAL, "null pointer");
     int rc = check_tensors(count, src, dst, numel, dtype);
     if (rc) return rc;
-    for (const Table &t : make_tables(count, src, dst, numel, dtype)) scale_kernel<<<blocks_of(t), kThreads, 0, st>>>(t, nullptr, 0, 0, max_norm, const_cast<float *>(norm));
+    for (const Table &t : make_tables(count, src, dst, numel, dtype)) scale_kernel<SHTB200_NORM_L2><<<blocks_of(t), kThreads, 0, st>>>(t, nullptr, 0, max_norm, const_cast<float *>(norm));
     SHT_CUDA_CHECK(cudaGetLastError());
     return SHTB200_OK;
 }

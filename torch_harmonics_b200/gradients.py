@@ -11,11 +11,15 @@ and hand the joined norm to ``clip_grads_with_norm_``.
 
 import math
 from array import array
+from operator import attrgetter
 from typing import Iterable, Tuple, Union
 
 import torch
 
 from . import _lib
+
+_get_grad, _get_dtype = attrgetter("grad"), attrgetter("dtype")
+_get_device, _is_contiguous, _data_ptr, _numel = torch.Tensor.get_device, torch.Tensor.is_contiguous, torch.Tensor.data_ptr, torch.Tensor.numel
 
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.complex64: _lib.C64}
 
@@ -49,7 +53,8 @@ def _fills_memory(t):
     return True
 
 
-def _check(tensors, what):
+def _refuse(tensors, what):
+    """Raise for the first tensor that cannot be taken."""
     for t in tensors:
         if not t.is_cuda:
             raise RuntimeError(f"{what}: expected CUDA tensors; torch_harmonics_b200 has no CPU path")
@@ -62,40 +67,57 @@ def _check(tensors, what):
 
 
 class _List:
-    """The tensors of a call as host arrays for the C ABI."""
+    """The tensors of a call, checked, gapless in memory, and as host arrays for the C ABI.
 
-    def __init__(self, tensors):
+    There may be hundreds of them on every step, and each look at an attribute costs a good part of a microsecond: the checks go through
+    the list a few times at C speed, and say which tensor was wrong only once one is."""
+
+    def __init__(self, tensors, what):
+        if set(map(_get_device, tensors)) != {tensors[0].get_device()} or tensors[0].get_device() < 0:
+            _refuse(tensors, what)
+        try:
+            self.types = [_DTYPES[t] for t in map(_get_dtype, tensors)]
+            self.tensors = tensors
+            if not all(map(_is_contiguous, tensors)):
+                _refuse(tensors, what)
+                # (a slice of a larger tensor is taken as a copy)
+                self.tensors = [t if _fills_memory(t) else t.contiguous() for t in tensors]
+            pointers = array("Q", map(_data_ptr, self.tensors))
+        except (KeyError, RuntimeError):  # (some layouts raise where they have no strides or no pointer)
+            _refuse(tensors, what)
+            raise
+        self.device = tensors[0].device
         self.n = len(tensors)
-        self._src = array("Q", [t.data_ptr() for t in tensors])
-        self._numel = array("q", [t.numel() for t in tensors])
-        self._dtype = array("i", [_DTYPES[t.dtype] for t in tensors])
-        self.src, self.numel, self.dtype = (a.buffer_info()[0] for a in (self._src, self._numel, self._dtype))
+        self._keep = (pointers, array("q", map(_numel, self.tensors)), array("i", self.types))
+        self.src, self.numel, self.dtype = (a.buffer_info()[0] for a in self._keep)
 
 
-def _norm(tensors, kind):
-    dev = tensors[0].device
-    lib, ls = _lib.load(), _List(tensors)
+def _workspace(lib, ls):
     nbytes = lib.shtb200_grad_norm_workspace_bytes(ls.n)
-    ws, norm = torch.empty(nbytes, dtype=torch.uint8, device=dev), torch.empty((), dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        rc = lib.shtb200_grad_norm(ls.n, ls.src, ls.numel, ls.dtype, kind, norm.data_ptr(), ws.data_ptr(), nbytes, torch.cuda.current_stream(dev).cuda_stream)
+    return torch.empty(nbytes, dtype=torch.uint8, device=ls.device), nbytes, torch.empty((), dtype=torch.float32, device=ls.device)
+
+
+def _norm(ls, kind):
+    lib = _lib.load()
+    with torch.cuda.device(ls.device):
+        ws, nbytes, norm = _workspace(lib, ls)
+        rc = lib.shtb200_grad_norm(ls.n, ls.src, ls.numel, ls.dtype, kind, norm.data_ptr(), ws.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream)
     _lib.check(rc, "shtb200_grad_norm")
     return norm
 
 
-def _clip(src, dst, max_norm, kind, norm=None):
-    """dst = src clipped; returns the norm, which is computed unless it is given."""
-    dev = src[0].device
-    lib, ls = _lib.load(), _List(src)
-    to = ls._src if dst is src else array("Q", [t.data_ptr() for t in dst])
-    with torch.cuda.device(dev):
-        stream = torch.cuda.current_stream(dev).cuda_stream
+def _clip(ls, dst, max_norm, kind, norm=None):
+    """dst = the tensors of ``ls`` clipped (``None``: in place); returns the norm, which is computed unless it is given."""
+    lib = _lib.load()
+    keep = None if dst is None else array("Q", map(_data_ptr, dst))
+    to = ls.src if dst is None else keep.buffer_info()[0]
+    with torch.cuda.device(ls.device):
+        stream = torch.cuda.current_stream().cuda_stream
         if norm is not None:
-            rc = lib.shtb200_scale_grads(ls.n, ls.src, to.buffer_info()[0], ls.numel, ls.dtype, max_norm, norm.data_ptr(), stream)
+            rc = lib.shtb200_scale_grads(ls.n, ls.src, to, ls.numel, ls.dtype, max_norm, norm.data_ptr(), stream)
         else:
-            nbytes = lib.shtb200_grad_norm_workspace_bytes(ls.n)
-            ws, norm = torch.empty(nbytes, dtype=torch.uint8, device=dev), torch.empty((), dtype=torch.float32, device=dev)
-            rc = lib.shtb200_clip_grads(ls.n, ls.src, to.buffer_info()[0], ls.numel, ls.dtype, kind, max_norm, norm.data_ptr(), ws.data_ptr(), nbytes, stream)
+            ws, nbytes, norm = _workspace(lib, ls)
+            rc = lib.shtb200_clip_grads(ls.n, ls.src, to, ls.numel, ls.dtype, kind, max_norm, norm.data_ptr(), ws.data_ptr(), nbytes, stream)
     _lib.check(rc, "shtb200_clip_grads")
     return norm
 
@@ -105,20 +127,18 @@ def _refuse_nonfinite(norm, norm_type):
         raise RuntimeError(f"The total norm of order {float(norm_type)} of the gradients is non-finite, so it cannot be clipped.")
 
 
-def _grads(parameters, what):
+def _grads(parameters):
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    grads = [p.grad for p in parameters if p.grad is not None]
-    _check(grads, what)
-    return grads
+    return [g for g in map(_get_grad, parameters) if g is not None]
 
 
-def _clip_in_place(grads, max_norm, kind, norm=None):
-    held = [g if _fills_memory(g) else g.contiguous() for g in grads]  # (a slice of a larger tensor is clipped in a copy)
-    norm = _clip(held, held, max_norm, kind, norm)
-    for g, h in zip(grads, held):
-        if h is not g:
-            g.copy_(h)
+def _clip_in_place(grads, ls, max_norm, kind, norm=None):
+    norm = _clip(ls, None, max_norm, kind, norm)
+    if ls.tensors is not grads:
+        for g, h in zip(grads, ls.tensors):
+            if h is not g:
+                g.copy_(h)
     torch.autograd.graph.increment_version(grads)
     return norm
 
@@ -128,10 +148,9 @@ def global_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type:
     """The norm of all entries of ``tensors`` together (``norm_type`` 2 or inf), a float32 scalar; zero for no tensors."""
     kind = _norm_kind(norm_type)
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    _check(tensors, "global_norm")
     if not tensors:
         return torch.tensor(0.0)
-    return _norm([t if _fills_memory(t) else t.contiguous() for t in tensors], kind)
+    return _norm(_List(tensors, "global_norm"), kind)
 
 
 @torch.no_grad()
@@ -143,26 +162,27 @@ def clip_grad_norm_(
     Parameters without a gradient are left out; gradients that share memory are refused.  A norm that is not finite makes the gradients zero or NaN, or
     raises with ``error_if_nonfinite`` (which waits for the device), before any gradient is touched."""
     kind, max_norm = _norm_kind(norm_type), _limit(max_norm)
-    grads = _grads(parameters, "clip_grad_norm_")
+    grads = _grads(parameters)
     if not grads:
         return torch.tensor(0.0)
-    norm = None
+    ls, norm = _List(grads, "clip_grad_norm_"), None
     if error_if_nonfinite:
-        norm = global_norm(grads, norm_type)
+        norm = _norm(ls, kind)
         _refuse_nonfinite(norm, norm_type)
-    return _clip_in_place(grads, max_norm, kind, norm)
+    return _clip_in_place(grads, ls, max_norm, kind, norm)
 
 
 @torch.no_grad()
 def clip_grads_with_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, total_norm: torch.Tensor) -> None:
     """``clip_grad_norm_`` with a norm that is known: a scalar on the gradients' device, e.g. one joined over several processes."""
     max_norm = _limit(max_norm)
-    grads = _grads(parameters, "clip_grads_with_norm_")
+    grads = _grads(parameters)
     if not grads:
         return
+    ls = _List(grads, "clip_grads_with_norm_")
     if total_norm.numel() != 1 or total_norm.device != grads[0].device:
         raise RuntimeError(f"clip_grads_with_norm_: expected total_norm as a scalar on {grads[0].device}, got shape {tuple(total_norm.shape)} on {total_norm.device}")
-    _clip_in_place(grads, max_norm, _lib.NORM_L2, total_norm.to(torch.float32).contiguous())
+    _clip_in_place(grads, ls, max_norm, _lib.NORM_L2, total_norm.to(torch.float32).contiguous())
 
 
 @torch.no_grad()
@@ -173,14 +193,13 @@ def clip_by_global_norm(
     (the gradients that ``torch.autograd.grad`` returns, or those of one micro-batch before they are accumulated)."""
     kind, max_norm = _norm_kind(norm_type), _limit(max_norm)
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    _check(tensors, "clip_by_global_norm")
     if not tensors:
         return (), torch.tensor(0.0)
-    src = [t.resolve_conj().resolve_neg() if _fills_memory(t) else _lib.dense(t) for t in tensors]
-    norm = None
+    tensors = [t.resolve_conj().resolve_neg() for t in tensors]
+    ls, norm = _List(tensors, "clip_by_global_norm"), None
     if error_if_nonfinite:
-        norm = _norm(src, kind)
+        norm = _norm(ls, kind)
         _refuse_nonfinite(norm, norm_type)
-    dst = [torch.empty_like(t) for t in src]
-    norm = _clip(src, dst, max_norm, kind, norm)
+    dst = [torch.empty_like(t) for t in ls.tensors]
+    norm = _clip(ls, dst, max_norm, kind, norm)
     return tuple(dst), norm
