@@ -28,6 +28,11 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _aligned(t):
+    """The kernels read 16 bytes at a time: a view that begins in between is copied."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _run(module, x, weight, bias):
     """y and what the backward pass needs, for a dense ``x``."""
     desc, nbytes, _ = module._call(x)
@@ -63,7 +68,7 @@ class _GroupNorm(torch.autograd.Function):
         if x.shape[0] == 0:
             return dx, dw, db, None
         # the gradient comes in any layout (an expanded scalar, for a sum): the kernel reads it in the layout of x
-        dy = _lib.dense(dy) if not desc.channels_last else dy.resolve_neg().contiguous(memory_format=torch.channels_last)
+        dy = _aligned(_lib.dense(dy) if not desc.channels_last else dy.resolve_neg().contiguous(memory_format=torch.channels_last))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
         with torch.cuda.device(x.device):
             rc = _lib.load().shtb200_group_norm_backward(
@@ -185,6 +190,7 @@ class GroupNormS2(nn.Module):
             raise RuntimeError(f"GroupNormS2: the input is on {x.device}, the latitude weights on {self.lat_weights.device}")
         if not (x.is_contiguous() or x.is_contiguous(memory_format=torch.channels_last)) or x.is_neg():
             x = _lib.dense(x)
+        x = _aligned(x)
         if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and (weight.requires_grad or bias.requires_grad))):
             return _GroupNorm.apply(x, weight, bias, self)
         return _run(self, x, weight, bias)[0]
