@@ -460,6 +460,61 @@ template <int K, int N> __device__ __forceinline__ void column_sums(const GnArgs
 }
 __device__ __forceinline__ float half_of(const F2 *tot, int pair, int col, int h) { return reinterpret_cast<const float *>(tot + pair * kMaxCols + col)[h]; }
 
+// A thread's vectors on their way: rounds of U vectors (of each tensor), R rounds ahead, through a ring of its own in shared memory.  Nobody
+// else reads it, so no barrier is needed; and what is in flight does not cost registers.
+template <int TENSORS, int U, int R> struct Feed {
+    static constexpr size_t bytes = (size_t)TENSORS * U * R * kThreads * 16;
+    uint32_t ring;                 // the thread's vector 0
+    const char *at[TENSORS];
+    long long step;
+    int left, slot;                // vectors to be sent for; the round at hand
+    __device__ __forceinline__ void send(int to) {
+        if (left >= U) {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int t = 0; t < TENSORS; ++t) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ring + 16u * kThreads * (uint32_t)((to * U + u) * TENSORS + t)), "l"(at[t]) : "memory");
+                    at[t] += step;
+                }
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (u < left)
+#pragma unroll
+                    for (int t = 0; t < TENSORS; ++t) {
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ring + 16u * kThreads * (uint32_t)((to * U + u) * TENSORS + t)), "l"(at[t]) : "memory");
+                        at[t] += step;
+                    }
+        }
+        left -= U;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    __device__ __forceinline__ void start(void *shared, const void *x, const void *y, int count, int step_vectors) {
+        ring = (uint32_t)__cvta_generic_to_shared(shared) + 16u * threadIdx.x;
+        at[0] = reinterpret_cast<const char *>(x);
+        if constexpr (TENSORS == 2) at[1] = reinterpret_cast<const char *>(y);
+        step = 16LL * step_vectors;
+        left = count;
+        slot = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i) send(i);
+    }
+    __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(R - 1) : "memory"); }
+    __device__ __forceinline__ uint4 get(int u, int t) const {
+        uint4 v;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "r"(ring + 16u * kThreads * (uint32_t)((slot * U + u) * TENSORS + t))
+                     : "memory");
+        return v;
+    }
+    __device__ __forceinline__ void next() {  // after the last get() of a round
+        send(slot);
+        if (++slot == R) slot = 0;
+    }
+};
+
 // What follows a launch waits here for it; what precedes it in the kernel overlaps its end.
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
@@ -483,8 +538,9 @@ __device__ __forceinline__ void recentre(F2 W, F2 delta, F2 &S1, F2 &S2) {
     S1 = sub2(S1, t);
 }
 
-constexpr int kUnroll = 4;
+constexpr int kUnroll = 2;
 constexpr int kStatsCtas = 4;  // on an SM
+using StatsFeed = Feed<1, kUnroll, 3>;
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, kStatsCtas) gn_stats_kernel(const __grid_constant__ GnArgs a) {
@@ -494,7 +550,8 @@ __global__ void __launch_bounds__(kThreads, kStatsCtas) gn_stats_kernel(const __
     __shared__ float centre[V * kMaxCols];
     // weights of a slot beyond its thread's common ones, where vectors lie across rows: rare, and registers are short
     F2(*extra)[kThreads] = reinterpret_cast<F2(*)[kThreads]>(red);
-    extern __shared__ Moments acc[];
+    extern __shared__ __align__(16) unsigned char gn_smem[];
+    Moments *acc = reinterpret_cast<Moments *>(gn_smem + StatsFeed::bytes);
     const Chunk k = make_chunk<T>(a, blockIdx.x);
     const T *x = reinterpret_cast<const T *>(a.x) + k.base;
     const uint4 *xv = reinterpret_cast<const uint4 *>(x + k.head);
@@ -511,26 +568,32 @@ __global__ void __launch_bounds__(kThreads, kStatsCtas) gn_stats_kernel(const __
             c[p] = q[p] = q[P + p] = f2(0.f);
             extra[p][threadIdx.x] = f2(0.f);
         }
+        StatsFeed feed;
+        feed.start(gn_smem, xv + s.first, nullptr, s.count, s.step);
         if (s.count) {
-            const uint4 *at = xv + s.first;
-            const int step = s.step;
             Rows r{0, 0, 0};
             if (a.lat) r = make_rows<T>(a, k, s, 0);
-            // The first centre: of the first round, the vector that counts most (a value at the pole, far out, is then no centre for
-            // rows of a hundred times its weight).
-            unpack(__ldg(at + (a.lat && 2 * r.row < a.nlat ? (long long)(min(U, s.count) - 1) * step : 0)), c, T());
             for (int j = 0; j < s.count; j += U) {
                 const int have = min(U, s.count - j);
                 uint4 raw[U];
                 float w[U];
                 bool plain = true;
                 const Rows r0 = r;
+                feed.wait();
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    raw[u] = make_uint4(0, 0, 0, 0);
-                    if (u < have) raw[u] = __ldg(at + (long long)u * step);
+                for (int u = 0; u < U; ++u) raw[u] = feed.get(u, 0);
+                // The first centre: of the first round, the vector that counts most (a value at the pole, far out, is then no centre for
+                // rows of a hundred times its weight).
+                if (j == 0) {
+                    if (a.lat && 2 * r.row < a.nlat) {
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+                            if (u < have) unpack(raw[u], c, T());
+                    } else {
+                        unpack(raw[0], c, T());
+                    }
                 }
-                at += (long long)U * step;
+                feed.next();
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     w[u] = 1.f;
@@ -735,7 +798,8 @@ __global__ void __launch_bounds__(kThreads) gn_finish_stats_kernel(const __grid_
     let_next_begin();
 }
 
-constexpr int kApplyCtas = 3;  // on an SM
+constexpr int kApplyCtas = 4;  // on an SM
+using ApplyFeed = Feed<1, 2, 6>;
 
 // Scale and shift of a slot.  float32: z = (x - m) sc + sh, the difference first, so that a level far above the spread costs nothing.
 // 16-bit values carry that error many times over themselves: z = x sc + sh, m in the shift.
@@ -743,8 +807,9 @@ template <typename T> constexpr bool kCentred = sizeof(T) == 4;
 
 template <typename T, int ACT>
 __global__ void __launch_bounds__(kThreads, kApplyCtas) gn_apply_kernel(const __grid_constant__ GnArgs a) {
-    constexpr int V = kV<T>, P = kP<T>, U = kUnroll;
-    extern __shared__ float4 st[];
+    constexpr int V = kV<T>, P = kP<T>, U = 2;
+    extern __shared__ __align__(16) unsigned char gn_smem[];
+    float4 *st = reinterpret_cast<float4 *>(gn_smem + ApplyFeed::bytes);
     const Chunk k = make_chunk<T>(a, a.tasks - 1 - (int)blockIdx.x);
     const T *x = reinterpret_cast<const T *>(a.x) + k.base;
     T *y = reinterpret_cast<T *>(a.out) + k.base;
@@ -752,6 +817,8 @@ __global__ void __launch_bounds__(kThreads, kApplyCtas) gn_apply_kernel(const __
     uint4 *yv = reinterpret_cast<uint4 *>(y + k.head);
     for (int win = 0; win < a.windows; ++win) {
         const Share s = make_share<T>(a, k, win);
+        ApplyFeed feed;
+        feed.start(gn_smem, xv + s.first, nullptr, s.count, s.step);  // (x was complete before the sums)
         F2 m[kCentred<T> ? P : 1], sc[P], sh[P];
         {
             float w[V], b[V];
@@ -771,7 +838,6 @@ __global__ void __launch_bounds__(kThreads, kApplyCtas) gn_apply_kernel(const __
             }
         }
         const long long step = s.step;
-        const uint4 *at = xv + s.first;
         uint4 *to = yv + s.first;
         auto one = [&](uint4 raw) {
             F2 v[P];
@@ -783,21 +849,15 @@ __global__ void __launch_bounds__(kThreads, kApplyCtas) gn_apply_kernel(const __
             }
             return pack(v, T());
         };
-        int j = 0;
-        for (; j + U <= s.count; j += U) {
+        for (int j = 0; j < s.count; j += U) {
+            feed.wait();
             uint4 raw[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) raw[u] = __ldg(at + u * step);
-#pragma unroll
-            for (int u = 0; u < U; ++u) to[u * step] = one(raw[u]);
-            at += U * step;
+            for (int u = 0; u < U; ++u) raw[u] = feed.get(u, 0);
+            feed.next();
+            to[0] = one(raw[0]);
+            if (j + 1 < s.count) to[step] = one(raw[1]);
             to += U * step;
-        }
-#pragma unroll 1
-        for (; j < s.count; ++j) {
-            *to = one(__ldg(at));
-            at += step;
-            to += step;
         }
     }
     if ((int)threadIdx.x < 2 * V) {
@@ -816,6 +876,7 @@ __global__ void __launch_bounds__(kThreads, kApplyCtas) gn_apply_kernel(const __
 // ------------------------------------------------------------------------------------------------
 constexpr int kUnrollB = 2;
 constexpr int kBackwardCtas = 3;  // on an SM
+using BackwardFeed = Feed<2, kUnrollB, 3>;
 
 __device__ __forceinline__ void load_stats(const GnArgs &a, const Chunk &k, float4 *st) {
     if (a.cl)
@@ -835,7 +896,8 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_sums_kernel(const 
     constexpr int V = kV<T>, P = kP<T>, U = kUnrollB;
     __shared__ __align__(16) F2 red[P * kThreads];
     __shared__ __align__(16) F2 tot[2 * P * kMaxCols];
-    extern __shared__ float4 st[];
+    extern __shared__ __align__(16) unsigned char gn_smem[];
+    float4 *st = reinterpret_cast<float4 *>(gn_smem + BackwardFeed::bytes);
     float2 *acc = reinterpret_cast<float2 *>(st + a.gu);
     const Chunk k = make_chunk<T>(a, blockIdx.x);
     const T *x = reinterpret_cast<const T *>(a.x) + k.base, *dy = reinterpret_cast<const T *>(a.dy) + k.base;
@@ -848,6 +910,8 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_sums_kernel(const 
     __syncthreads();
     for (int win = 0; win < a.windows; ++win) {
         const Share s = make_share<T>(a, k, win);
+        BackwardFeed feed;
+        feed.start(gn_smem, xv + s.first, dv + s.first, s.count, s.step);
         F2 q[2 * P], m[P], sc[P], sh[P];  // q: sum g, sum g (x - m)
         {
             float w[V], b[V];
@@ -862,8 +926,6 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_sums_kernel(const 
                 q[p] = q[P + p] = f2(0.f);
             }
         }
-        const long long step = s.step;
-        const uint4 *ax = xv + s.first, *ad = dv + s.first;
         auto one = [&](uint4 rx, uint4 rd) {
             F2 v[P], d[P];
             unpack(rx, v, T());
@@ -875,24 +937,17 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_sums_kernel(const 
                 q[P + p] = fma2(g, e, q[P + p]);
             }
         };
-        int j = 0;
-        for (; j + U <= s.count; j += U) {
+        for (int j = 0; j < s.count; j += U) {
+            feed.wait();
             uint4 rx[U], rd[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                rx[u] = __ldg(ax + u * step);
-                rd[u] = __ldg(ad + u * step);
+                rx[u] = feed.get(u, 0);
+                rd[u] = feed.get(u, 1);
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u) one(rx[u], rd[u]);
-            ax += U * step;
-            ad += U * step;
-        }
-#pragma unroll 1
-        for (; j < s.count; ++j) {
-            one(__ldg(ax), __ldg(ad));
-            ax += step;
-            ad += step;
+            feed.next();
+            one(rx[0], rd[0]);
+            if (j + 1 < s.count) one(rx[1], rd[1]);
         }
         if (a.cu == 1) {
             float v[2];
@@ -1008,29 +1063,36 @@ __device__ void group_sums(const GnArgs &a, const Chunk &k, float2 *gsum) {
         if (lane == 0) gsum[0] = make_float2((float)t.x, (float)t.y);
     }
 }
-// ... the sums of the channels joined once: a CTA for 32 channels of a sample, a lane each, the chunks dealt to the warps
+// ... the sums of the channels joined once: a CTA for 4 channels of a sample (32 bytes of every chunk), the chunks dealt to 64 lanes a channel
+constexpr int kFinishChannels = 4;
 __global__ void __launch_bounds__(kThreads) gn_finish_sums_kernel(const __grid_constant__ GnArgs a) {
-    __shared__ double2 red[kThreads];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, blocks = (a.C + 31) / 32, b = blockIdx.x / blocks, c = (blockIdx.x - b * blocks) * 32 + lane;
+    __shared__ double2 red[kWarps * kFinishChannels];
+    const int blocks = (a.C + kFinishChannels - 1) / kFinishChannels, b = blockIdx.x / blocks;
+    const int i = threadIdx.x % kFinishChannels, first = threadIdx.x / kFinishChannels, c = (blockIdx.x - b * blocks) * kFinishChannels + i;
+    constexpr int kRows = kThreads / kFinishChannels;
     wait_for_previous();
     double2 v = make_double2(0., 0.);
     if (c < a.C)
-        for (int n = warp; n < a.chunks; n += 8 * kWarps) {
+        for (int n = first; n < a.chunks; n += 8 * kRows) {
             float2 p[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) p[u] = n + u * kWarps < a.chunks ? __ldcg(a.bpart + ((long long)b * a.chunks + n + u * kWarps) * a.C + c) : make_float2(0.f, 0.f);
+            for (int u = 0; u < 8; ++u) p[u] = n + u * kRows < a.chunks ? __ldcg(a.bpart + ((long long)b * a.chunks + n + u * kRows) * a.C + c) : make_float2(0.f, 0.f);
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 v.x += p[u].x;
                 v.y += p[u].y;
             }
         }
-    red[threadIdx.x] = v;
+    for (int o = 16; o >= kFinishChannels; o >>= 1) {
+        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+        v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    }
+    if ((threadIdx.x & 31) < kFinishChannels) red[(threadIdx.x >> 5) * kFinishChannels + i] = v;
     __syncthreads();
-    if (warp == 0 && c < a.C) {
+    if (threadIdx.x < kFinishChannels && c < a.C) {
         for (int w = 1; w < kWarps; ++w) {
-            v.x += red[w * 32 + lane].x;
-            v.y += red[w * 32 + lane].y;
+            v.x += red[w * kFinishChannels + i].x;
+            v.y += red[w * kFinishChannels + i].y;
         }
         a.csum[(long long)b * a.C + c] = v;
     }
@@ -1070,7 +1132,8 @@ __device__ __forceinline__ float2 group_terms(const float4 &v, const float2 &t) 
 template <typename T, int ACT>
 __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_dx_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kUnrollB;
-    extern __shared__ float4 st[];
+    extern __shared__ __align__(16) unsigned char gn_smem[];
+    float4 *st = reinterpret_cast<float4 *>(gn_smem + BackwardFeed::bytes);
     float2 *gsum = reinterpret_cast<float2 *>(st + a.gu);
     const int tasks = a.out ? a.tasks : 0;
     if ((int)blockIdx.x >= tasks) {
@@ -1083,12 +1146,16 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_dx_kernel(const __
     T *dx = reinterpret_cast<T *>(a.out) + k.base;
     const uint4 *xv = reinterpret_cast<const uint4 *>(x + k.head), *dv = reinterpret_cast<const uint4 *>(dy + k.head);
     uint4 *ov = reinterpret_cast<uint4 *>(dx + k.head);
-    wait_for_previous();
-    load_stats(a, k, st);
-    group_sums(a, k, gsum);
-    __syncthreads();
     for (int win = 0; win < a.windows; ++win) {
         const Share s = make_share<T>(a, k, win);
+        BackwardFeed feed;
+        feed.start(gn_smem, xv + s.first, dv + s.first, s.count, s.step);  // (x and dy were complete before the sums)
+        if (win == 0) {
+            wait_for_previous();
+            load_stats(a, k, st);
+            group_sums(a, k, gsum);
+            __syncthreads();
+        }
         F2 m[kCentred<T> ? P : 1], sc[P], sh[P], al[P], be[P];
         {
             float w[V], b[V];
@@ -1112,7 +1179,6 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_dx_kernel(const __
         }
         if (!s.count) continue;
         const long long step = s.step;
-        const uint4 *ax = xv + s.first, *ad = dv + s.first;
         uint4 *to = ov + s.first;
         Rows r{0, 0, 0};
         if (a.lat) r = make_rows<T>(a, k, s, 0);
@@ -1135,14 +1201,13 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_dx_kernel(const __
             float w[U];
             bool plain = true;
             const Rows r0 = r;
+            feed.wait();
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                rx[u] = rd[u] = make_uint4(0, 0, 0, 0);
-                if (u < have) {
-                    rx[u] = __ldg(ax + u * step);
-                    rd[u] = __ldg(ad + u * step);
-                }
+                rx[u] = feed.get(u, 0);
+                rd[u] = feed.get(u, 1);
             }
+            feed.next();
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 w[u] = 1.f;
@@ -1170,8 +1235,6 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_dx_kernel(const __
                     }
                     to[u * step] = one(rx[u], rd[u], wt);
                 }
-            ax += U * step;
-            ad += U * step;
             to += U * step;
         }
     }
@@ -1337,9 +1400,9 @@ int group_norm_forward(const GroupNormDesc *d, const void *x, const float *lat, 
     a.bias = bias;
     a.stats = reinterpret_cast<float4 *>(stats);
     a.part = reinterpret_cast<float4 *>(ws);
-    if ((rc = launch(kernel_for<Stats>(*d), a.tasks, a.cu > 1 ? sizeof(Moments) * a.gu : 0, a, st))) return rc;
+    if ((rc = launch(kernel_for<Stats>(*d), a.tasks, StatsFeed::bytes + (a.cu > 1 ? sizeof(Moments) * a.gu : 0), a, st))) return rc;
     if (!a.direct && (rc = launch((const void *)gn_finish_stats_kernel, a.B * a.G, 0, a, st))) return rc;
-    return launch(kernel_for<Apply>(*d), a.tasks, sizeof(float4) * a.gu, a, st);
+    return launch(kernel_for<Apply>(*d), a.tasks, ApplyFeed::bytes + sizeof(float4) * a.gu, a, st);
 }
 
 int group_norm_backward(const GroupNormDesc *d, const void *dy, const void *x, const float *lat, const void *weight, const void *bias, const void *stats, void *dx, void *dweight,
@@ -1365,9 +1428,9 @@ int group_norm_backward(const GroupNormDesc *d, const void *dy, const void *x, c
     a.csum = reinterpret_cast<double2 *>(reinterpret_cast<char *>(ws) + l.part);
     const int grads = dweight || dbias ? ceil_div(a.C, kWarps) : 0;
     if (!dx && !grads) return SHTB200_OK;
-    const size_t smem = sizeof(float4) * a.gu + sizeof(float2) * std::max(a.cu, a.gu);
+    const size_t smem = BackwardFeed::bytes + sizeof(float4) * a.gu + sizeof(float2) * std::max(a.cu, a.gu);
     if ((rc = launch(kernel_for<SumsOf>(*d), a.tasks, smem, a, st))) return rc;
-    if (!a.direct && (rc = launch((const void *)gn_finish_sums_kernel, a.B * ceil_div(a.C, 32), 0, a, st))) return rc;
+    if (!a.direct && (rc = launch((const void *)gn_finish_sums_kernel, a.B * ceil_div(a.C, kFinishChannels), 0, a, st))) return rc;
     return launch(kernel_for<Dx>(*d), (dx ? a.tasks : 0) + grads, smem, a, st);
 }
 
