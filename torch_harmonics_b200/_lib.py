@@ -117,6 +117,30 @@ def load():
         return lib
 
 
+class on_device:
+    """``with on_device(index) as stream``: make a CUDA device current, unless it is already (which costs next to nothing); the device's
+    current stream as an integer."""
+
+    __slots__ = ("index", "previous")
+
+    def __init__(self, index):
+        self.index = index
+
+    def __enter__(self):
+        import torch
+
+        self.previous = torch._C._cuda_getDevice()
+        if self.previous != self.index:
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.previous != self.index:
+            import torch
+
+            torch.cuda.set_device(self.previous)
+
+
 def check(rc, what):
     if rc != 0:
         msg = load().shtb200_last_error().decode("utf-8", "replace")

@@ -82,7 +82,8 @@ __device__ __forceinline__ float rcp_fast(float x) {
 // ------------------------------------------------------------------------------------------------
 // Normal distribution function of -|z|:  Phi(-a) = e^(-a^2 / 2) R(a),  R(a) = t P(t) with t = 1 / (1 + 0.3 a): the polynomial P of
 // degree 7 is the minimax fit of R(a) / t in relative error over 0 <= a <= 13.5 (1.3e-7; computed by reweighted least squares
-// against the scaled complementary error function).  gelu(z) = max(z, 0) - a Phi(-a) then keeps its relative accuracy in both tails.
+// against the scaled complementary error function).  Values that are rounded to 16 bits behind it take degree 5 and 1 / (1 + 0.31 a) (4.6e-6, a
+// hundredth of float16's half step).  gelu(z) = max(z, 0) - a Phi(-a) then keeps its relative accuracy in both tails.
 struct Tail {
     F2 e, r, na;  // e^(-a^2 / 2), R(a), -a
 };
@@ -109,6 +110,9 @@ __device__ __forceinline__ F2 logistic(F2 z) {
     return f2(rcp_fast(d.x), rcp_fast(d.y));
 }
 
+// (gelu behind 16-bit rounding takes kValueScale z:  y = z / 2 - a (1/2 - e^(-a^2 / 2) R(a)), two operations less; what this loses of the
+// far tail, 1e-7 |z|, is far below the rounding)
+template <typename T, int ACT> constexpr float kValueScale = ACT == SHTB200_ACT_GELU && sizeof(T) == 2 ? 0.84932180f : 1.f;
 template <typename T, int ACT> __device__ __forceinline__ F2 act_value(F2 z) {
     if constexpr (ACT == SHTB200_ACT_RELU) {
         const float2 v = split(z);
@@ -116,24 +120,57 @@ template <typename T, int ACT> __device__ __forceinline__ F2 act_value(F2 z) {
     } else if constexpr (ACT == SHTB200_ACT_SILU) {
         return mul2(z, logistic(z));
     } else if constexpr (ACT == SHTB200_ACT_GELU) {
-        const Tail k = normal_tail(z);
-        const float2 v = split(z);
-        return fma2(k.na, mul2(k.e, k.r), f2(fmaxf(v.x, 0.f), fmaxf(v.y, 0.f)));
+        if constexpr (sizeof(T) == 2) {
+            constexpr float F = 1.f / kValueScale<T, ACT>;
+            F2 na;
+            na.v = z.v | 0x8000000080000000ull;
+            const float2 d = split(fma2(na, f2(-0.31f * F), f2(1.f)));
+            const F2 t = f2(rcp_fast(d.x), rcp_fast(d.y));
+            F2 r = fma2(t, f2(-0.07392906f * F), f2(0.1804501f * F));
+            r = fma2(t, r, f2(0.015744982f * F));
+            r = fma2(t, r, f2(0.13342965f * F));
+            r = fma2(t, r, f2(0.12044131f * F));
+            r = fma2(t, r, f2(0.1238607f * F));
+            const float2 x = split(mul2(z, z));
+            return fma2(na, fma2(f2(exp2_fast(-x.x), exp2_fast(-x.y)), mul2(t, r), f2(-0.5f * F)), mul2(z, f2(0.5f * F)));
+        } else {
+            const Tail k = normal_tail(z);
+            const float2 v = split(z);
+            return fma2(k.na, mul2(k.e, k.r), f2(fmaxf(v.x, 0.f), fmaxf(v.y, 0.f)));
+        }
     }
     return z;
 }
-template <int ACT> __device__ __forceinline__ F2 act_slope(F2 z) {
+// The slope takes kSlopeScale z, which costs nothing where z is made from a scale and a shift, and comes divided by it again (OVER) where a scale
+// follows.  gelu'(z) = Phi(z) + z phi(z) = 1/2 + sign(z) (1/2 - e^(-a^2 / 2) (R(a) - a / sqrt(2 pi))), here with e^(-a^2 / 2) = 2^(-zs^2) and
+// R fitted (as above) in absolute error weighted by e^(-a^2 / 2): degree 5 with t = 1 / (1 + 0.28 a), 2.0e-7 over all z in float32 arithmetic.
+template <int ACT> constexpr float kSlopeScale = ACT == SHTB200_ACT_GELU ? 0.84932180f : ACT == SHTB200_ACT_SILU ? 1.44269504f : 1.f;
+template <int ACT, bool OVER> __device__ __forceinline__ F2 act_slope(F2 zs) {
+    constexpr float F = OVER ? 1.f / kSlopeScale<ACT> : 1.f;
     if constexpr (ACT == SHTB200_ACT_RELU) {
-        const float2 v = split(z);
+        const float2 v = split(zs);
         return f2(v.x <= 0.f ? 0.f : 1.f, v.y <= 0.f ? 0.f : 1.f);
     } else if constexpr (ACT == SHTB200_ACT_SILU) {
-        const F2 s = logistic(z);
-        return fma2(mul2(z, s), fma2(s, f2(-1.f), f2(1.f)), s);
+        constexpr float kLn2 = 0.69314718f * F;
+        const float2 x = split(zs);
+        const float2 d = split(add2(f2(exp2_fast(-x.x), exp2_fast(-x.y)), f2(1.f)));
+        const F2 s = f2(rcp_fast(d.x), rcp_fast(d.y));
+        return fma2(mul2(zs, s), fma2(s, f2(-kLn2), f2(kLn2)), OVER ? mul2(s, f2(F)) : s);
     } else if constexpr (ACT == SHTB200_ACT_GELU) {
-        const Tail k = normal_tail(z);
-        const F2 s = mul2(k.e, fma2(k.na, f2(0.39894228f), k.r));  // the slope at -a; at a it is one less this
-        const float2 m = split(s), p = split(fma2(s, f2(-1.f), f2(1.f))), v = split(z);
-        return f2(v.x > 0.f ? p.x : m.x, v.y > 0.f ? p.y : m.y);
+        F2 na;
+        na.v = zs.v | 0x8000000080000000ull;
+        const float2 d = split(fma2(na, f2(-0.3296748f), f2(1.f)));
+        const F2 t = f2(rcp_fast(d.x), rcp_fast(d.y));
+        F2 r = fma2(t, f2(0.101911396f * F), f2(-0.37383756f * F));
+        r = fma2(t, r, f2(0.21076515f * F));
+        r = fma2(t, r, f2(-0.24760479f * F));
+        r = fma2(t, r, f2(-0.07608968f * F));
+        r = fma2(t, r, f2(-0.11514454f * F));
+        r = fma2(na, f2(-0.46971864f * F), mul2(t, r));  // a / sqrt(2 pi) - R(a)
+        const float2 x = split(mul2(zs, zs));
+        F2 h = fma2(f2(exp2_fast(-x.x), exp2_fast(-x.y)), r, f2(0.5f * F));
+        h.v ^= zs.v & 0x8000000080000000ull;
+        return add2(h, f2(0.5f * F));
     }
     return f2(1.f);
 }
@@ -229,11 +266,11 @@ struct GnArgs {
     int B, C, G, cg, nlat, nlon, cl, pdtype;
     float eps;
     int cu, gu, cgu;   // channels, groups of a unit, channels of a group inside a unit: (C, G, cg) channels last, (1, 1, 1) for planes
-    int chunks, chunk_px;         // of a unit
-    int tasks;                    // chunks of all units
+    int chunks, chunk_px, tasks;  // of a unit for the sums; chunks of all units
+    int chunks2, chunk_px2, tasks2;  // the same for the second pass
     int cols, dup;                // lcm(cu, V) / V: vectors after which the channels repeat; how often each occurs in them
     int win_cols, windows, reps;  // columns a CTA covers at a time, how many windows that takes, vectors of a column it takes side by side
-    int step_rows, step_cols;     // reps periods further in pixels, as rows and columns of the grid
+    int step_px, step_rows, step_cols;  // from a thread's vector to its next, in pixels, and as rows and columns of the grid
     int lanes;                    // that join the slots of a group
     int direct;        // the partial results of a group are joined by every CTA that needs them; else by a launch in between
 };
@@ -245,14 +282,14 @@ struct Chunk {
     int px0;         // its pixel
     int n, head, vecs;
 };
-template <typename T> __device__ __forceinline__ Chunk make_chunk(const GnArgs &a, int task) {
+template <typename T> __device__ __forceinline__ Chunk make_chunk(const GnArgs &a, int task, int chunks, int chunk_px) {
     Chunk k;
-    k.unit = (int)((unsigned)task / (unsigned)a.chunks);
-    k.chunk = task - k.unit * a.chunks;
+    k.unit = (int)((unsigned)task / (unsigned)chunks);
+    k.chunk = task - k.unit * chunks;
     k.b = a.cl ? k.unit : (int)((unsigned)k.unit / (unsigned)a.C);
     k.c = a.cl ? 0 : k.unit - k.b * a.C;
-    k.px0 = k.chunk * a.chunk_px;
-    const int px = (int)min((long long)a.chunk_px, a.hw - k.px0);
+    k.px0 = k.chunk * chunk_px;
+    const int px = (int)min((long long)chunk_px, a.hw - k.px0);
     k.base = ((long long)k.unit * a.hw + k.px0) * a.cu;
     k.n = px * a.cu;
     const unsigned mis = (unsigned)((uintptr_t)(reinterpret_cast<const T *>(a.x) + k.base) & 15u);
@@ -267,13 +304,22 @@ struct Share {
 };
 template <typename T> __device__ __forceinline__ Share make_share(const GnArgs &a, const Chunk &k, int window) {
     Share s;
+    if (a.cu == 1) {  // planes: a contiguous stretch for every warp, so that a thread stays in a row for a while
+        const int per = (k.vecs + kThreads - 1) / kThreads * 32, lo = (int)(threadIdx.x >> 5) * per, hi = min(lo + per, k.vecs);
+        s.rep = threadIdx.x;
+        s.col = s.ch0 = 0;
+        s.first = lo + (int)(threadIdx.x & 31);
+        s.step = 32;
+        s.count = s.first < hi ? (hi - s.first + 31) / 32 : 0;
+        return s;
+    }
     s.rep = a.win_cols == 1 ? (int)threadIdx.x : (int)(threadIdx.x / (unsigned)a.win_cols);
     s.col = (int)threadIdx.x - s.rep * a.win_cols;
     const int c = window * a.win_cols + s.col;
     s.first = c + s.rep * a.cols;
     s.step = a.reps * a.cols;
     s.count = (s.rep < a.reps && c < a.cols && s.first < k.vecs) ? (int)((unsigned)(k.vecs - s.first + s.step - 1) / (unsigned)s.step) : 0;
-    s.ch0 = a.cu == 1 ? 0 : (int)((unsigned)(c * kV<T> + k.head) % (unsigned)a.cu);
+    s.ch0 = (int)((unsigned)(c * kV<T> + k.head) % (unsigned)a.cu);
     return s;
 }
 
@@ -539,11 +585,11 @@ __device__ __forceinline__ void recentre(F2 W, F2 delta, F2 &S1, F2 &S2) {
 }
 
 constexpr int kUnroll = 2;
-constexpr int kStatsCtas = 4;  // on an SM
+template <typename T> constexpr int kStatsCtas = sizeof(T) == 4 ? 4 : 3;  // on an SM: 8 slots a thread need more registers than 4
 using StatsFeed = Feed<1, kUnroll, 3>;
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, kStatsCtas) gn_stats_kernel(const __grid_constant__ GnArgs a) {
+__global__ void __launch_bounds__(kThreads, kStatsCtas<T>) gn_stats_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kUnroll;
     __shared__ __align__(16) F2 red[P * kThreads];
     __shared__ __align__(16) F2 tot[3 * P * kMaxCols];
@@ -552,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, kStatsCtas) gn_stats_kernel(const __
     F2(*extra)[kThreads] = reinterpret_cast<F2(*)[kThreads]>(red);
     extern __shared__ __align__(16) unsigned char gn_smem[];
     Moments *acc = reinterpret_cast<Moments *>(gn_smem + StatsFeed::bytes);
-    const Chunk k = make_chunk<T>(a, blockIdx.x);
+    const Chunk k = make_chunk<T>(a, blockIdx.x, a.chunks, a.chunk_px);
     const T *x = reinterpret_cast<const T *>(a.x) + k.base;
     const uint4 *xv = reinterpret_cast<const uint4 *>(x + k.head);
     float4 *out = a.part + ((long long)k.unit * a.chunks + k.chunk) * a.gu;
@@ -572,70 +618,60 @@ __global__ void __launch_bounds__(kThreads, kStatsCtas) gn_stats_kernel(const __
         feed.start(gn_smem, xv + s.first, nullptr, s.count, s.step);
         if (s.count) {
             Rows r{0, 0, 0};
-            if (a.lat) r = make_rows<T>(a, k, s, 0);
+            float w = 1.f;
+            if (a.lat) {
+                r = make_rows<T>(a, k, s, 0);
+                w = __ldg(a.lat + r.row);
+            }
             for (int j = 0; j < s.count; j += U) {
                 const int have = min(U, s.count - j);
                 uint4 raw[U];
-                float w[U];
-                bool plain = true;
-                const Rows r0 = r;
                 feed.wait();
 #pragma unroll
                 for (int u = 0; u < U; ++u) raw[u] = feed.get(u, 0);
                 // The first centre: of the first round, the vector that counts most (a value at the pole, far out, is then no centre for
                 // rows of a hundred times its weight).
                 if (j == 0) {
-                    if (a.lat && 2 * r.row < a.nlat) {
-#pragma unroll
-                        for (int u = 0; u < U; ++u)
-                            if (u < have) unpack(raw[u], c, T());
-                    } else {
-                        unpack(raw[0], c, T());
-                    }
+                    unpack(raw[0], c, T());
+                    if (a.lat && 2 * r.row < a.nlat && have == U) unpack(raw[U - 1], c, T());
                 }
                 feed.next();
+                if (have == U && (!a.lat || r.col + U * a.step_px + r.over < a.nlon)) {  // all in one row, the next one too
+                    const F2 w2 = f2(w);
+                    F2 wp[P];
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    w[u] = 1.f;
-                    if (a.lat && u < have) {
-                        w[u] = __ldg(a.lat + r.row);
-                        plain = plain && r.col + r.over < a.nlon;
-                        advance(a, r);
-                    }
-                }
-                if (plain && have == U) {
+                    for (int p = 0; p < P; ++p) wp[p] = w2;
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
-                        F2 v[P], wp[P];
+                        F2 v[P];
                         unpack(raw[u], v, T());
-#pragma unroll
-                        for (int p = 0; p < P; ++p) wp[p] = f2(w[u]);
                         accumulate<T>(v, c, q, wp);
-                        W += w[u];
                     }
+                    W = fmaf((float)U, w, W);
+                    r.col += U * a.step_px;
                 } else {
-                    Rows n = r0;
 #pragma unroll
                     for (int u = 0; u < U; ++u)
                         if (u < have) {
                             F2 v[P], wp[P];
                             unpack(raw[u], v, T());
 #pragma unroll
-                            for (int p = 0; p < P; ++p) wp[p] = f2(w[u]);
-                            if (a.lat) {
-                                if (n.col + n.over >= a.nlon) {
-                                    float ws[V];
-                                    mixed_weights<T>(a.lat, a.nlon, a.cu, s.ch0, n.row, n.col, ws);
+                            for (int p = 0; p < P; ++p) wp[p] = f2(w);
+                            if (a.lat && r.col + r.over >= a.nlon) {
+                                float ws[V];
+                                mixed_weights<T>(a.lat, a.nlon, a.cu, s.ch0, r.row, r.col, ws);
 #pragma unroll
-                                    for (int p = 0; p < P; ++p) {
-                                        wp[p] = f2(ws[2 * p], ws[2 * p + 1]);
-                                        extra[p][threadIdx.x] = add2(extra[p][threadIdx.x], sub2(wp[p], f2(w[u])));
-                                    }
+                                for (int p = 0; p < P; ++p) {
+                                    wp[p] = f2(ws[2 * p], ws[2 * p + 1]);
+                                    extra[p][threadIdx.x] = add2(extra[p][threadIdx.x], sub2(wp[p], f2(w)));
                                 }
-                                advance(a, n);
                             }
                             accumulate<T>(v, c, q, wp);
-                            W += w[u];
+                            W += w;
+                            if (a.lat) {
+                                advance(a, r);
+                                w = __ldg(a.lat + min(r.row, a.nlat - 1));
+                            }
                         }
                 }
                 const int round = j / U;
@@ -746,31 +782,32 @@ __global__ void __launch_bounds__(kThreads, kStatsCtas) gn_stats_kernel(const __
     let_next_begin();
 }
 
+// The partial results of a group: n of them, stride apart.
+__device__ __forceinline__ void group_parts(const GnArgs &a, int b, int g, const float4 **p, int *n, int *stride) {
+    *p = a.cl ? a.part + (long long)b * a.chunks * a.G + g : a.part + ((long long)b * a.C + g * a.cg) * a.chunks;
+    *n = a.cl ? a.chunks : a.cg * a.chunks;
+    *stride = a.cl ? a.G : 1;
+}
+
 // Statistics of the groups of a chunk's unit, into shared memory.  Where they are joined here (the same order in every CTA), no launch in between is
 // needed.
 __device__ __forceinline__ void unit_stats(const GnArgs &a, const Chunk &k, float4 *st) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (!a.cl) {
-        if (warp == 0) {
-            const int g = (int)((unsigned)k.c / (unsigned)a.cg), first = k.b * a.C + g * a.cg;
+    const int g0 = a.cl ? 0 : (int)((unsigned)k.c / (unsigned)a.cg);  // first group of the unit
+    if (a.direct) {
+        for (int i = warp; i < a.gu; i += kWarps) {
+            const float4 *p;
+            int n, stride;
+            group_parts(a, k.b, g0 + i, &p, &n, &stride);
             Sums64 m;
-            m.gather(a.part + (long long)first * a.chunks, a.cg * a.chunks, 1, lane, 32);
+            m.gather(p, n, stride, lane, 32);
             if (lane == 0) {
-                st[0] = m.stats(a);
-                if (k.unit == first && k.chunk == 0) a.stats[k.b * a.G + g] = st[0];
-            }
-        }
-    } else if (a.direct) {
-        for (int g = warp; g < a.G; g += kWarps) {
-            Sums64 m;
-            m.gather(a.part + (long long)k.b * a.chunks * a.G + g, a.chunks, a.G, lane, 32);
-            if (lane == 0) {
-                st[g] = m.stats(a);
-                if (k.chunk == 0) a.stats[k.b * a.G + g] = st[g];
+                st[i] = m.stats(a);
+                if (k.chunk == 0 && (a.cl || k.c == g0 * a.cg)) a.stats[k.b * a.G + g0 + i] = st[i];
             }
         }
     } else {
-        for (int g = threadIdx.x; g < a.G; g += kThreads) st[g] = __ldcg(a.stats + (long long)k.b * a.G + g);
+        for (int i = threadIdx.x; i < a.gu; i += kThreads) st[i] = __ldcg(a.stats + (long long)k.b * a.G + g0 + i);
     }
     __syncthreads();
 }
@@ -780,7 +817,10 @@ __global__ void __launch_bounds__(kThreads) gn_finish_stats_kernel(const __grid_
     const int warp = threadIdx.x >> 5, b = blockIdx.x / a.G, g = blockIdx.x - b * a.G;
     wait_for_previous();
     Sums64 m;
-    m.gather(a.part + (long long)b * a.chunks * a.G + g, a.chunks, a.G, threadIdx.x, kThreads);
+    const float4 *p;
+    int n, stride;
+    group_parts(a, b, g, &p, &n, &stride);
+    m.gather(p, n, stride, threadIdx.x, kThreads);
     if ((threadIdx.x & 31) == 0) {
         red[warp * 3] = m.W;
         red[warp * 3 + 1] = m.s;
@@ -799,7 +839,8 @@ __global__ void __launch_bounds__(kThreads) gn_finish_stats_kernel(const __grid_
 }
 
 constexpr int kApplyCtas = 4;  // on an SM
-using ApplyFeed = Feed<1, 2, 6>;
+constexpr int kApplyUnroll = 2;
+using ApplyFeed = Feed<1, kApplyUnroll, 6>;
 
 // Scale and shift of a slot.  float32: z = (x - m) sc + sh, the difference first, so that a level far above the spread costs nothing.
 // 16-bit values carry that error many times over themselves: z = x sc + sh, m in the shift.
@@ -807,10 +848,10 @@ template <typename T> constexpr bool kCentred = sizeof(T) == 4;
 
 template <typename T, int ACT>
 __global__ void __launch_bounds__(kThreads, kApplyCtas) gn_apply_kernel(const __grid_constant__ GnArgs a) {
-    constexpr int V = kV<T>, P = kP<T>, U = 2;
+    constexpr int V = kV<T>, P = kP<T>, U = kApplyUnroll;
     extern __shared__ __align__(16) unsigned char gn_smem[];
     float4 *st = reinterpret_cast<float4 *>(gn_smem + ApplyFeed::bytes);
-    const Chunk k = make_chunk<T>(a, a.tasks - 1 - (int)blockIdx.x);
+    const Chunk k = make_chunk<T>(a, a.tasks2 - 1 - (int)blockIdx.x, a.chunks2, a.chunk_px2);
     const T *x = reinterpret_cast<const T *>(a.x) + k.base;
     T *y = reinterpret_cast<T *>(a.out) + k.base;
     const uint4 *xv = reinterpret_cast<const uint4 *>(x + k.head);
@@ -831,8 +872,9 @@ __global__ void __launch_bounds__(kThreads, kApplyCtas) gn_apply_kernel(const __
 #pragma unroll
             for (int p = 0; p < P; ++p) {
                 const float4 u = st[g[2 * p]], v = st[g[2 * p + 1]];
-                sc[p] = mul2(f2(u.z, v.z), f2(w[2 * p], w[2 * p + 1]));
-                sh[p] = fma2(f2(-u.y, -v.y), sc[p], f2(b[2 * p], b[2 * p + 1]));
+                constexpr float F = kValueScale<T, ACT>;
+                sc[p] = mul2(f2(u.z * F, v.z * F), f2(w[2 * p], w[2 * p + 1]));
+                sh[p] = fma2(f2(-u.y, -v.y), sc[p], f2(b[2 * p] * F, b[2 * p + 1] * F));
                 if constexpr (kCentred<T>) m[p] = f2(u.x, v.x);
                 else sh[p] = fma2(f2(-u.x, -v.x), sc[p], sh[p]);
             }
@@ -855,8 +897,14 @@ __global__ void __launch_bounds__(kThreads, kApplyCtas) gn_apply_kernel(const __
 #pragma unroll
             for (int u = 0; u < U; ++u) raw[u] = feed.get(u, 0);
             feed.next();
-            to[0] = one(raw[0]);
-            if (j + 1 < s.count) to[step] = one(raw[1]);
+            if (j + U <= s.count) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) to[u * step] = one(raw[u]);
+            } else {
+#pragma unroll
+                for (int u = 0; u < U - 1; ++u)
+                    if (j + u < s.count) to[u * step] = one(raw[u]);
+            }
             to += U * step;
         }
     }
@@ -866,7 +914,7 @@ __global__ void __launch_bounds__(kThreads, kApplyCtas) gn_apply_kernel(const __
             const int ch = e % a.cu, c = a.cl ? ch : k.c;
             const float4 v = st[ch / a.cgu];
             const float sc = v.z * load_param(a.weight, a.pdtype, c, 1.f), sh = fmaf(-v.y, sc, load_param(a.bias, a.pdtype, c, 0.f));
-            store_f(y + e, split(act_value<T, ACT>(f2(fmaf(to_f(x[e]) - v.x, sc, sh)))).x);
+            store_f(y + e, split(act_value<T, ACT>(f2(kValueScale<T, ACT> * fmaf(to_f(x[e]) - v.x, sc, sh)))).x);
         }
     }
 }
@@ -875,8 +923,8 @@ __global__ void __launch_bounds__(kThreads, kApplyCtas) gn_apply_kernel(const __
 // backward
 // ------------------------------------------------------------------------------------------------
 constexpr int kUnrollB = 2;
-constexpr int kBackwardCtas = 3;  // on an SM
-using BackwardFeed = Feed<2, kUnrollB, 3>;
+constexpr int kBackwardCtas = 2;  // on an SM: what a thread keeps of 8 slots and the activation's constants spills at 3 (361x720x256 bf16 164 us, at 2 139 us)
+using BackwardFeed = Feed<2, kUnrollB, 4>;
 
 __device__ __forceinline__ void load_stats(const GnArgs &a, const Chunk &k, float4 *st) {
     if (a.cl)
@@ -888,7 +936,7 @@ template <typename T, int ACT> __device__ __forceinline__ float2 ragged_slope(co
     const int c = a.cl ? ch : k.c;
     const float4 v = st[ch / a.cgu];
     const float sc = v.z * load_param(a.weight, a.pdtype, c, 1.f), sh = fmaf(-v.y, sc, load_param(a.bias, a.pdtype, c, 0.f)), d = x - v.x;
-    return make_float2(dy * split(act_slope<ACT>(f2(fmaf(d, sc, sh)))).x, d);
+    return make_float2(dy * split(act_slope<ACT, false>(f2(kSlopeScale<ACT> * fmaf(d, sc, sh)))).x, d);
 }
 
 template <typename T, int ACT>
@@ -899,7 +947,7 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_sums_kernel(const 
     extern __shared__ __align__(16) unsigned char gn_smem[];
     float4 *st = reinterpret_cast<float4 *>(gn_smem + BackwardFeed::bytes);
     float2 *acc = reinterpret_cast<float2 *>(st + a.gu);
-    const Chunk k = make_chunk<T>(a, blockIdx.x);
+    const Chunk k = make_chunk<T>(a, blockIdx.x, a.chunks, a.chunk_px);
     const T *x = reinterpret_cast<const T *>(a.x) + k.base, *dy = reinterpret_cast<const T *>(a.dy) + k.base;
     const uint4 *xv = reinterpret_cast<const uint4 *>(x + k.head), *dv = reinterpret_cast<const uint4 *>(dy + k.head);
     float2 *out = a.bpart + ((long long)k.unit * a.chunks + k.chunk) * a.cu;
@@ -921,8 +969,8 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_sums_kernel(const 
             for (int p = 0; p < P; ++p) {
                 const float4 u = st[g[2 * p]], v = st[g[2 * p + 1]];
                 m[p] = f2(u.x, v.x);
-                sc[p] = mul2(f2(u.z, v.z), f2(w[2 * p], w[2 * p + 1]));
-                sh[p] = fma2(f2(-u.y, -v.y), sc[p], f2(b[2 * p], b[2 * p + 1]));
+                sc[p] = mul2(f2(u.z * kSlopeScale<ACT>, v.z * kSlopeScale<ACT>), f2(w[2 * p], w[2 * p + 1]));
+                sh[p] = fma2(f2(-u.y, -v.y), sc[p], f2(b[2 * p] * kSlopeScale<ACT>, b[2 * p + 1] * kSlopeScale<ACT>));
                 q[p] = q[P + p] = f2(0.f);
             }
         }
@@ -932,7 +980,7 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_sums_kernel(const 
             unpack(rd, d, T());
 #pragma unroll
             for (int p = 0; p < P; ++p) {
-                const F2 e = sub2(v[p], m[p]), g = mul2(d[p], act_slope<ACT>(fma2(e, sc[p], sh[p])));
+                const F2 e = sub2(v[p], m[p]), g = mul2(d[p], act_slope<ACT, false>(fma2(e, sc[p], sh[p])));
                 q[p] = add2(q[p], g);
                 q[P + p] = fma2(g, e, q[P + p]);
             }
@@ -1015,8 +1063,10 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_sums_kernel(const 
 // (sum h, sum h xh) of the groups of a chunk's unit
 __device__ void group_sums(const GnArgs &a, const Chunk &k, float2 *gsum) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (a.cl) {
-        for (int g = warp; g < a.G; g += kWarps) {
+    if (a.cl || !a.direct) {
+        const int g0 = a.cl ? 0 : (int)((unsigned)k.c / (unsigned)a.cg);  // first group of the unit
+        for (int j = warp; j < a.gu; j += kWarps) {
+            const int g = g0 + j;
             double2 t = make_double2(0., 0.);
             if (a.direct) {
                 for (int i = lane; i < a.cg * a.chunks; i += 32) {
@@ -1036,7 +1086,7 @@ __device__ void group_sums(const GnArgs &a, const Chunk &k, float2 *gsum) {
                 }
             }
             t = warp_sum(t);
-            if (lane == 0) gsum[g] = make_float2((float)t.x, (float)t.y);
+            if (lane == 0) gsum[j] = make_float2((float)t.x, (float)t.y);
         }
     } else if (warp == 0) {
         const int first = k.c - (int)((unsigned)k.c % (unsigned)a.cg);  // first channel of the group
@@ -1076,7 +1126,7 @@ __global__ void __launch_bounds__(kThreads) gn_finish_sums_kernel(const __grid_c
         for (int n = first; n < a.chunks; n += 8 * kRows) {
             float2 p[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) p[u] = n + u * kRows < a.chunks ? __ldcg(a.bpart + ((long long)b * a.chunks + n + u * kRows) * a.C + c) : make_float2(0.f, 0.f);
+            for (int u = 0; u < 8; ++u) p[u] = n + u * kRows < a.chunks ? __ldcg(a.bpart + (a.cl ? ((long long)b * a.chunks + n + u * kRows) * a.C + c : ((long long)b * a.C + c) * a.chunks + n + u * kRows)) : make_float2(0.f, 0.f);
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 v.x += p[u].x;
@@ -1135,13 +1185,13 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_dx_kernel(const __
     extern __shared__ __align__(16) unsigned char gn_smem[];
     float4 *st = reinterpret_cast<float4 *>(gn_smem + BackwardFeed::bytes);
     float2 *gsum = reinterpret_cast<float2 *>(st + a.gu);
-    const int tasks = a.out ? a.tasks : 0;
+    const int tasks = a.out ? a.tasks2 : 0;
     if ((int)blockIdx.x >= tasks) {
         wait_for_previous();
         parameter_gradients(a, blockIdx.x - tasks);
         return;
     }
-    const Chunk k = make_chunk<T>(a, tasks - 1 - (int)blockIdx.x);
+    const Chunk k = make_chunk<T>(a, tasks - 1 - (int)blockIdx.x, a.chunks2, a.chunk_px2);
     const T *x = reinterpret_cast<const T *>(a.x) + k.base, *dy = reinterpret_cast<const T *>(a.dy) + k.base;
     T *dx = reinterpret_cast<T *>(a.out) + k.base;
     const uint4 *xv = reinterpret_cast<const uint4 *>(x + k.head), *dv = reinterpret_cast<const uint4 *>(dy + k.head);
@@ -1165,8 +1215,8 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_dx_kernel(const __
             for (int p = 0; p < P; ++p) {
                 const float4 u = st[g[2 * p]], v = st[g[2 * p + 1]];
                 const float2 tu = group_terms(u, gsum[g[2 * p]]), tv = group_terms(v, gsum[g[2 * p + 1]]);
-                sc[p] = mul2(f2(u.z, v.z), f2(w[2 * p], w[2 * p + 1]));
-                sh[p] = fma2(f2(-u.y, -v.y), sc[p], f2(b[2 * p], b[2 * p + 1]));
+                sc[p] = mul2(f2(u.z * kSlopeScale<ACT>, v.z * kSlopeScale<ACT>), f2(w[2 * p], w[2 * p + 1]));
+                sh[p] = fma2(f2(-u.y, -v.y), sc[p], f2(b[2 * p] * kSlopeScale<ACT>, b[2 * p + 1] * kSlopeScale<ACT>));
                 al[p] = f2(tu.x, tv.x);
                 be[p] = f2(tu.y, tv.y);
                 if constexpr (kCentred<T>) {
@@ -1181,7 +1231,11 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_dx_kernel(const __
         const long long step = s.step;
         uint4 *to = ov + s.first;
         Rows r{0, 0, 0};
-        if (a.lat) r = make_rows<T>(a, k, s, 0);
+        float w = 1.f;
+        if (a.lat) {
+            r = make_rows<T>(a, k, s, 0);
+            w = __ldg(a.lat + r.row);
+        }
         auto one = [&](uint4 rx, uint4 rd, const F2 (&wt)[P]) {
             F2 v[P], d[P];
             unpack(rx, v, T());
@@ -1190,7 +1244,7 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_dx_kernel(const __
             for (int p = 0; p < P; ++p) {
                 F2 e = v[p];
                 if constexpr (kCentred<T>) e = sub2(e, m[p]);
-                const F2 g = mul2(d[p], act_slope<ACT>(fma2(e, sc[p], sh[p])));
+                const F2 g = mul2(d[p], act_slope<ACT, true>(fma2(e, sc[p], sh[p])));
                 v[p] = fma2(wt[p], fma2(e, be[p], al[p]), mul2(sc[p], g));
             }
             return pack(v, T());
@@ -1198,9 +1252,6 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_dx_kernel(const __
         for (int j = 0; j < s.count; j += U) {
             const int have = min(U, s.count - j);
             uint4 rx[U], rd[U];
-            float w[U];
-            bool plain = true;
-            const Rows r0 = r;
             feed.wait();
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -1208,33 +1259,33 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_dx_kernel(const __
                 rd[u] = feed.get(u, 1);
             }
             feed.next();
+            F2 wt[P];
+            if (have == U && (!a.lat || r.col + U * a.step_px + r.over < a.nlon)) {  // all in one row, the next one too
+                const F2 w2 = f2(w);
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                w[u] = 1.f;
-                if (a.lat && u < have) {
-                    w[u] = __ldg(a.lat + r.row);
-                    plain = plain && r.col + r.over < a.nlon;
-                    advance(a, r);
-                }
-            }
-            Rows n = r0;
+                for (int p = 0; p < P; ++p) wt[p] = w2;
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (u < have) {
-                    F2 wt[P];
+                for (int u = 0; u < U; ++u) to[u * step] = one(rx[u], rd[u], wt);
+                r.col += U * a.step_px;
+            } else {
 #pragma unroll
-                    for (int p = 0; p < P; ++p) wt[p] = f2(w[u]);
-                    if (!plain) {
-                        if (n.col + n.over >= a.nlon) {
+                for (int u = 0; u < U; ++u)
+                    if (u < have) {
+#pragma unroll
+                        for (int p = 0; p < P; ++p) wt[p] = f2(w);
+                        if (a.lat && r.col + r.over >= a.nlon) {
                             float ws[V];
-                            mixed_weights<T>(a.lat, a.nlon, a.cu, s.ch0, n.row, n.col, ws);
+                            mixed_weights<T>(a.lat, a.nlon, a.cu, s.ch0, r.row, r.col, ws);
 #pragma unroll
                             for (int p = 0; p < P; ++p) wt[p] = f2(ws[2 * p], ws[2 * p + 1]);
                         }
-                        advance(a, n);
+                        to[u * step] = one(rx[u], rd[u], wt);
+                        if (a.lat) {
+                            advance(a, r);
+                            w = __ldg(a.lat + min(r.row, a.nlat - 1));
+                        }
                     }
-                    to[u * step] = one(rx[u], rd[u], wt);
-                }
+            }
             to += U * step;
         }
     }
@@ -1253,7 +1304,7 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_dx_kernel(const __
 // host
 // ------------------------------------------------------------------------------------------------
 constexpr int kMaxChannels = 4096;  // what a CTA keeps per channel or group has to fit into its shared memory
-constexpr int kDirect = 2048;       // partial results of a unit up to which every CTA joins them itself
+constexpr int kDirect = 128;        // partial results of a group up to which every CTA joins them itself, a warp a group, instead of a launch in between
 
 int value_bytes(int dtype) { return dtype == SHTB200_F32 ? 4 : 2; }
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
@@ -1264,6 +1315,20 @@ struct Launch {
     size_t part = 0, csum = 0;  // bytes of workspace
     size_t total() const { return part + csum; }
 };
+
+constexpr int kSumWaves = 1, kPassWaves = 2;
+
+// Chunks of a unit: `per_sm` CTAs for each of 148 SMs, but no chunk under 16 KB (what a CTA does besides costs some microseconds, which the
+// others on its SM have to cover).
+void cut(const GnArgs &a, int V, int per_sm, int *chunks, int *chunk_px, int *tasks) {
+    const int units = a.cl ? a.B : a.B * a.C;
+    const long long unit_vecs = a.hw * a.cu / V, most = std::max<long long>(1, std::min<long long>(a.hw, unit_vecs / (kThreads * 4)));
+    const long long n = std::min<long long>(most, std::max(1, per_sm * 148 / units));
+    *chunk_px = (int)((a.hw + n - 1) / n);
+    if (*chunk_px >= 256) *chunk_px = (*chunk_px + 31) / 32 * 32;  // (chunks of an aligned field begin aligned)
+    *chunks = (int)((a.hw + *chunk_px - 1) / *chunk_px);
+    *tasks = units * *chunks;
+}
 
 Launch geometry(const GroupNormDesc &d, bool backward) {
     Launch l;
@@ -1290,19 +1355,13 @@ Launch geometry(const GroupNormDesc &d, bool backward) {
     a.win_cols = ceil_div(a.cols, a.windows);
     a.reps = kThreads / a.win_cols;
     for (a.lanes = 1; a.lanes < 32 && a.lanes < a.cgu * a.dup;) a.lanes *= 2;
-    const long long step_px = (long long)a.reps * a.cols * V / a.cu;
+    const long long step_px = a.cu == 1 ? 32 * V : (long long)a.reps * a.cols * V / a.cu;
+    a.step_px = (int)step_px;
     a.step_rows = (int)(step_px / a.nlon);
     a.step_cols = (int)(step_px % a.nlon);
-    // Chunks: two waves of CTAs on 148 SMs and more, but none under 16 KB (the sums of a chunk cost some microseconds, which the other
-    // CTAs on the SM have to cover).
-    const int units = a.cl ? a.B : a.B * a.C;
-    const long long unit_vecs = a.hw * a.cu / V, most = std::max<long long>(1, std::min<long long>(a.hw, unit_vecs / (kThreads * 4)));
-    const long long chunks = std::min<long long>(most, std::max(1, 2 * 4 * 148 / units));
-    a.chunk_px = (int)((a.hw + chunks - 1) / chunks);
-    if (a.chunk_px >= 256) a.chunk_px = (a.chunk_px + 31) / 32 * 32;  // (chunks of an aligned field begin aligned)
-    a.chunks = (int)((a.hw + a.chunk_px - 1) / a.chunk_px);
-    a.tasks = units * a.chunks;
-    a.direct = !a.cl || (long long)a.chunks * (backward ? a.C : a.G) <= kDirect;
+    cut(a, V, (backward ? kBackwardCtas : V == 4 ? kStatsCtas<float> : kStatsCtas<__half>) * kSumWaves, &a.chunks, &a.chunk_px, &a.tasks);
+    cut(a, V, (backward ? kBackwardCtas : kApplyCtas) * kPassWaves, &a.chunks2, &a.chunk_px2, &a.tasks2);
+    a.direct = a.gu <= kWarps && (long long)a.chunks * (backward || !a.cl ? a.cg : 1) <= kDirect;
     l.part = up256((size_t)a.tasks * (backward ? a.cu * sizeof(float2) : a.gu * sizeof(float4)));
     if (backward && !a.direct) l.csum = up256((size_t)a.B * a.C * sizeof(double2));
     return l;
@@ -1369,7 +1428,7 @@ int plan(const GroupNormDesc *d, bool backward, const void *ws, size_t ws_bytes,
     if (!ws || ws_bytes < l->total()) return fail(SHTB200_EWORKSPACE, "workspace too small: need " + std::to_string(l->total()) + " bytes");
     if (((uintptr_t)ws & 255) != 0) return fail(SHTB200_EINVAL, "workspace must be 256-byte aligned");
     if (((uintptr_t)stats & 15) != 0) return fail(SHTB200_EINVAL, "the statistics must be 16-byte aligned");
-    if ((long long)l->a.chunk_px * l->a.cu > (1 << 30)) return fail(SHTB200_EINVAL, "group norm shape too large");
+    if ((long long)std::max(l->a.chunk_px, l->a.chunk_px2) * l->a.cu > (1 << 30)) return fail(SHTB200_EINVAL, "group norm shape too large");
     return SHTB200_OK;
 }
 // vectors are aligned in all tensors or in none
@@ -1402,7 +1461,7 @@ int group_norm_forward(const GroupNormDesc *d, const void *x, const float *lat, 
     a.part = reinterpret_cast<float4 *>(ws);
     if ((rc = launch(kernel_for<Stats>(*d), a.tasks, StatsFeed::bytes + (a.cu > 1 ? sizeof(Moments) * a.gu : 0), a, st))) return rc;
     if (!a.direct && (rc = launch((const void *)gn_finish_stats_kernel, a.B * a.G, 0, a, st))) return rc;
-    return launch(kernel_for<Apply>(*d), a.tasks, ApplyFeed::bytes + sizeof(float4) * a.gu, a, st);
+    return launch(kernel_for<Apply>(*d), a.tasks2, ApplyFeed::bytes + sizeof(float4) * a.gu, a, st);
 }
 
 int group_norm_backward(const GroupNormDesc *d, const void *dy, const void *x, const float *lat, const void *weight, const void *bias, const void *stats, void *dx, void *dweight,
@@ -1431,7 +1490,7 @@ int group_norm_backward(const GroupNormDesc *d, const void *dy, const void *x, c
     const size_t smem = BackwardFeed::bytes + sizeof(float4) * a.gu + sizeof(float2) * std::max(a.cu, a.gu);
     if ((rc = launch(kernel_for<SumsOf>(*d), a.tasks, smem, a, st))) return rc;
     if (!a.direct && (rc = launch((const void *)gn_finish_sums_kernel, a.B * ceil_div(a.C, kFinishChannels), 0, a, st))) return rc;
-    return launch(kernel_for<Dx>(*d), (dx ? a.tasks : 0) + grads, smem, a, st);
+    return launch(kernel_for<Dx>(*d), (dx ? a.tasks2 : 0) + grads, smem, a, st);
 }
 
 }  // namespace shtb200

@@ -20,6 +20,7 @@ from . import _lib
 
 _get_grad, _get_dtype = attrgetter("grad"), attrgetter("dtype")
 _get_device, _is_contiguous, _data_ptr, _numel = torch.Tensor.get_device, torch.Tensor.is_contiguous, torch.Tensor.data_ptr, torch.Tensor.numel
+_is_conj, _is_neg = torch.Tensor.is_conj, torch.Tensor.is_neg
 
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.complex64: _lib.C64}
 
@@ -99,9 +100,9 @@ def _workspace(lib, ls):
 
 def _norm(ls, kind):
     lib = _lib.load()
-    with torch.cuda.device(ls.device):
+    with _lib.on_device(ls.device.index) as stream:
         ws, nbytes, norm = _workspace(lib, ls)
-        rc = lib.shtb200_grad_norm(ls.n, ls.src, ls.numel, ls.dtype, kind, norm.data_ptr(), ws.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream)
+        rc = lib.shtb200_grad_norm(ls.n, ls.src, ls.numel, ls.dtype, kind, norm.data_ptr(), ws.data_ptr(), nbytes, stream)
     _lib.check(rc, "shtb200_grad_norm")
     return norm
 
@@ -111,8 +112,7 @@ def _clip(ls, dst, max_norm, kind, norm=None):
     lib = _lib.load()
     keep = None if dst is None else array("Q", map(_data_ptr, dst))
     to = ls.src if dst is None else keep.buffer_info()[0]
-    with torch.cuda.device(ls.device):
-        stream = torch.cuda.current_stream().cuda_stream
+    with _lib.on_device(ls.device.index) as stream:
         if norm is not None:
             rc = lib.shtb200_scale_grads(ls.n, ls.src, to, ls.numel, ls.dtype, max_norm, norm.data_ptr(), stream)
         else:
@@ -195,11 +195,12 @@ def clip_by_global_norm(
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not tensors:
         return (), torch.tensor(0.0)
-    tensors = [t.resolve_conj().resolve_neg() for t in tensors]
+    if any(map(_is_conj, tensors)) or any(map(_is_neg, tensors)):
+        tensors = [t.resolve_conj().resolve_neg() for t in tensors]
     ls, norm = _List(tensors, "clip_by_global_norm"), None
     if error_if_nonfinite:
         norm = _norm(ls, kind)
         _refuse_nonfinite(norm, norm_type)
-    dst = [torch.empty_like(t) for t in ls.tensors]
+    dst = list(map(torch.empty_like, ls.tensors))
     norm = _clip(ls, dst, max_norm, kind, norm)
     return tuple(dst), norm

@@ -33,26 +33,30 @@ def _aligned(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _run(module, x, weight, bias):
-    """y and what the backward pass needs, for a dense ``x``."""
-    desc, nbytes, _ = module._call(x)
+def _run(module, x, weight, bias, keep):
+    """y and (with ``keep``) what the backward pass needs, for a dense ``x``."""
+    desc, ws_bytes, _ = module._call(x)
+    batch, dev = x.shape[0], x.device
     y = torch.empty_like(x)
-    stats = torch.empty(x.shape[0], module.num_groups, 4, dtype=torch.float32, device=x.device)
-    if x.shape[0] == 0:
+    stats_bytes = (16 * batch * module.num_groups + 255) // 256 * 256
+    stats = torch.empty(stats_bytes if keep else stats_bytes + ws_bytes, dtype=torch.uint8, device=dev)
+    if batch == 0:
         return y, stats
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if keep else None
+    at = stats.data_ptr()
+    with _lib.on_device(dev.index) as stream:
         rc = _lib.load().shtb200_group_norm_forward(
-            desc, x.data_ptr(), _ptr(module.lat_weights), _ptr(weight), _ptr(bias), y.data_ptr(), stats.data_ptr(), ws.data_ptr(), nbytes, torch.cuda.current_stream(x.device).cuda_stream
+            desc, x.data_ptr(), _ptr(module.lat_weights), _ptr(weight), _ptr(bias), y.data_ptr(), at, ws.data_ptr() if keep else at + stats_bytes, ws_bytes, stream
         )
-    _lib.check(rc, "shtb200_group_norm_forward")
+    if rc != 0:
+        _lib.check(rc, "shtb200_group_norm_forward")
     return y, stats
 
 
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, module):
-        y, stats = _run(module, x, weight, bias)
+        y, stats = _run(module, x, weight, bias, True)
         ctx.save_for_backward(x, weight, bias, stats, module.lat_weights)
         ctx.call = module._call(x)
         return y
@@ -61,21 +65,23 @@ class _GroupNorm(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, weight, bias, stats, lat = ctx.saved_tensors
-        desc, _, nbytes = ctx.call
-        dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
-        dw = torch.zeros_like(weight) if ctx.needs_input_grad[1] else None
-        db = torch.zeros_like(bias) if ctx.needs_input_grad[2] else None
+        desc, _, ws_bytes = ctx.call
+        new = torch.empty_like if x.shape[0] else torch.zeros_like
+        need = ctx.needs_input_grad
+        dx = torch.empty_like(x) if need[0] else None
+        dw = new(weight) if need[1] else None
+        db = new(bias) if need[2] else None
         if x.shape[0] == 0:
             return dx, dw, db, None
         # the gradient comes in any layout (an expanded scalar, for a sum): the kernel reads it in the layout of x
         dy = _aligned(_lib.dense(dy) if not desc.channels_last else dy.resolve_neg().contiguous(memory_format=torch.channels_last))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        with torch.cuda.device(x.device):
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+        with _lib.on_device(x.device.index) as stream:
             rc = _lib.load().shtb200_group_norm_backward(
-                desc, dy.data_ptr(), x.data_ptr(), _ptr(lat), _ptr(weight), _ptr(bias), stats.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(), nbytes,
-                torch.cuda.current_stream(x.device).cuda_stream,
+                desc, dy.data_ptr(), x.data_ptr(), _ptr(lat), _ptr(weight), _ptr(bias), stats.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(), ws_bytes, stream
             )
-        _lib.check(rc, "shtb200_group_norm_backward")
+        if rc != 0:
+            _lib.check(rc, "shtb200_group_norm_backward")
         return dx, dw, db, None
 
 
@@ -193,4 +199,4 @@ class GroupNormS2(nn.Module):
         x = _aligned(x)
         if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and (weight.requires_grad or bias.requires_grad))):
             return _GroupNorm.apply(x, weight, bias, self)
-        return _run(self, x, weight, bias)[0]
+        return _run(self, x, weight, bias, False)[0]
