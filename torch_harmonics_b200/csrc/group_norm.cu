@@ -302,17 +302,16 @@ template <typename T> __device__ __forceinline__ Chunk make_chunk(const GnArgs &
 struct Share {
     int first, step, count, ch0, rep, col;
 };
-template <typename T> __device__ __forceinline__ Share make_share(const GnArgs &a, const Chunk &k, int window) {
+template <typename T, bool PLANES> __device__ __forceinline__ Share make_share(const GnArgs &a, const Chunk &k, int window) {
     Share s;
-    if (a.cu == 1) {  // planes: a contiguous stretch for every warp, so that a thread stays in a row for a while
+    if constexpr (PLANES) {  // a contiguous stretch for every warp, so that a thread stays in a row for a while
         const int per = (k.vecs + kThreads - 1) / kThreads * 32, lo = (int)(threadIdx.x >> 5) * per, hi = min(lo + per, k.vecs);
         s.rep = threadIdx.x;
         s.col = s.ch0 = 0;
         s.first = lo + (int)(threadIdx.x & 31);
         s.step = 32;
         s.count = s.first < hi ? (hi - s.first + 31) / 32 : 0;
-        return s;
-    }
+    } else {
     s.rep = a.win_cols == 1 ? (int)threadIdx.x : (int)(threadIdx.x / (unsigned)a.win_cols);
     s.col = (int)threadIdx.x - s.rep * a.win_cols;
     const int c = window * a.win_cols + s.col;
@@ -320,6 +319,7 @@ template <typename T> __device__ __forceinline__ Share make_share(const GnArgs &
     s.step = a.reps * a.cols;
     s.count = (s.rep < a.reps && c < a.cols && s.first < k.vecs) ? (int)((unsigned)(k.vecs - s.first + s.step - 1) / (unsigned)s.step) : 0;
     s.ch0 = (int)((unsigned)(c * kV<T> + k.head) % (unsigned)a.cu);
+    }
     return s;
 }
 
@@ -361,8 +361,8 @@ template <typename T> __device__ __forceinline__ int ragged(const Chunk &k, int 
 __device__ __forceinline__ float weight_at(const GnArgs &a, const Chunk &k, int e) { return a.lat ? __ldg(a.lat + (k.px0 + e / a.cu) / a.nlon) : 1.f; }
 
 // Weight, bias and group (of the unit) of the V slots from channel ch on.  The loads go out together.
-template <int V> __device__ __forceinline__ void slot_params(const GnArgs &a, const Chunk &k, int ch, float (&w)[V], float (&b)[V], int (&g)[V]) {
-    if (a.cu == 1) {
+template <int V, bool PLANES> __device__ __forceinline__ void slot_params(const GnArgs &a, const Chunk &k, int ch, float (&w)[V], float (&b)[V], int (&g)[V]) {
+    if constexpr (PLANES) {
         const float w0 = load_param(a.weight, a.pdtype, k.c, 1.f), b0 = load_param(a.bias, a.pdtype, k.c, 0.f);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -588,12 +588,12 @@ constexpr int kUnroll = 2;
 template <typename T> constexpr int kStatsCtas = sizeof(T) == 4 ? 4 : 3;  // on an SM: 8 slots a thread need more registers than 4
 using StatsFeed = Feed<1, kUnroll, 3>;
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, kStatsCtas<T>) gn_stats_kernel(const __grid_constant__ GnArgs a) {
+template <typename T, bool PLANES> __global__ void __launch_bounds__(kThreads, kStatsCtas<T>) gn_stats_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kUnroll;
     __shared__ __align__(16) F2 red[P * kThreads];
-    __shared__ __align__(16) F2 tot[3 * P * kMaxCols];
-    __shared__ float centre[V * kMaxCols];
+    __shared__ __align__(16) F2 tot[PLANES ? kWarps * 2 : 3 * P * kMaxCols];
+    __shared__ float centre[PLANES ? V : V * kMaxCols];
+    constexpr int kPitch = PLANES ? 1 : kMaxCols;
     // weights of a slot beyond its thread's common ones, where vectors lie across rows: rare, and registers are short
     F2(*extra)[kThreads] = reinterpret_cast<F2(*)[kThreads]>(red);
     extern __shared__ __align__(16) unsigned char gn_smem[];
@@ -602,11 +602,12 @@ __global__ void __launch_bounds__(kThreads, kStatsCtas<T>) gn_stats_kernel(const
     const T *x = reinterpret_cast<const T *>(a.x) + k.base;
     const uint4 *xv = reinterpret_cast<const uint4 *>(x + k.head);
     float4 *out = a.part + ((long long)k.unit * a.chunks + k.chunk) * a.gu;
-    if (a.cu > 1)
+    if (!PLANES)
         for (int g = threadIdx.x; g < a.gu; g += kThreads) acc[g] = {0.f, 0.f, 0.f, 0.f};
     wait_for_previous();
-    for (int win = 0; win < a.windows; ++win) {
-        const Share s = make_share<T>(a, k, win);
+    let_next_begin();
+    for (int win = 0; win < (PLANES ? 1 : a.windows); ++win) {
+        const Share s = make_share<T, PLANES>(a, k, win);
         F2 c[P], q[2 * P];
         float W = 0.f;
 #pragma unroll
@@ -692,20 +693,20 @@ __global__ void __launch_bounds__(kThreads, kStatsCtas<T>) gn_stats_kernel(const
         for (int p = 0; p < P; ++p) {
             const float2 v = split(c[p]);
             if (s.rep == 0) {
-                centre[(2 * p) * kMaxCols + s.col] = v.x;
-                centre[(2 * p + 1) * kMaxCols + s.col] = v.y;
+                centre[(2 * p) * kPitch + s.col] = v.x;
+                centre[(2 * p + 1) * kPitch + s.col] = v.y;
             }
             z[p] = add2(extra[p][threadIdx.x], f2(W));
         }
         __syncthreads();
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const F2 c0 = a.cu == 1 ? f2(centre[0]) : f2(centre[(2 * p) * kMaxCols + s.col], centre[(2 * p + 1) * kMaxCols + s.col]);
+            const F2 c0 = PLANES ? f2(centre[0]) : f2(centre[(2 * p) * kPitch + s.col], centre[(2 * p + 1) * kPitch + s.col]);
             if (s.count) recentre(z[p], sub2(c0, c[p]), q[p], q[P + p]);
             z[P + p] = q[p];
             z[2 * P + p] = q[P + p];
         }
-        if (a.cu == 1) {
+        if constexpr (PLANES) {
             float v[3];
 #pragma unroll
             for (int i = 0; i < 3; ++i) {
@@ -735,9 +736,7 @@ __global__ void __launch_bounds__(kThreads, kStatsCtas<T>) gn_stats_kernel(const
                 }
                 out[0] = make_float4(m.W, m.K, m.m, m.M2);
             }
-            let_next_begin();
-            return;
-        }
+        } else {
         column_sums<3, P>(a, s, z, red, tot);
         // groups: a few lanes each go through its channels' slots in this window
         const int period = a.cols * V, slots = a.cgu * a.dup, shift = k.head % a.cu, L = a.lanes;
@@ -778,8 +777,8 @@ __global__ void __launch_bounds__(kThreads, kStatsCtas<T>) gn_stats_kernel(const
             }
         }
         if (a.windows > 1) __syncthreads();
+        }
     }
-    let_next_begin();
 }
 
 // The partial results of a group: n of them, stride apart.
@@ -846,8 +845,7 @@ using ApplyFeed = Feed<1, kApplyUnroll, 6>;
 // 16-bit values carry that error many times over themselves: z = x sc + sh, m in the shift.
 template <typename T> constexpr bool kCentred = sizeof(T) == 4;
 
-template <typename T, int ACT>
-__global__ void __launch_bounds__(kThreads, kApplyCtas) gn_apply_kernel(const __grid_constant__ GnArgs a) {
+template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kThreads, kApplyCtas) gn_apply_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kApplyUnroll;
     extern __shared__ __align__(16) unsigned char gn_smem[];
     float4 *st = reinterpret_cast<float4 *>(gn_smem + ApplyFeed::bytes);
@@ -856,17 +854,18 @@ __global__ void __launch_bounds__(kThreads, kApplyCtas) gn_apply_kernel(const __
     T *y = reinterpret_cast<T *>(a.out) + k.base;
     const uint4 *xv = reinterpret_cast<const uint4 *>(x + k.head);
     uint4 *yv = reinterpret_cast<uint4 *>(y + k.head);
-    for (int win = 0; win < a.windows; ++win) {
-        const Share s = make_share<T>(a, k, win);
+    for (int win = 0; win < (PLANES ? 1 : a.windows); ++win) {
+        const Share s = make_share<T, PLANES>(a, k, win);
         ApplyFeed feed;
         feed.start(gn_smem, xv + s.first, nullptr, s.count, s.step);  // (x was complete before the sums)
         F2 m[kCentred<T> ? P : 1], sc[P], sh[P];
         {
             float w[V], b[V];
             int g[V];
-            slot_params<V>(a, k, s.ch0, w, b, g);
+            slot_params<V, PLANES>(a, k, s.ch0, w, b, g);
             if (win == 0) {
                 wait_for_previous();
+                let_next_begin();
                 unit_stats(a, k, st);
             }
 #pragma unroll
@@ -939,11 +938,10 @@ template <typename T, int ACT> __device__ __forceinline__ float2 ragged_slope(co
     return make_float2(dy * split(act_slope<ACT, false>(f2(kSlopeScale<ACT> * fmaf(d, sc, sh)))).x, d);
 }
 
-template <typename T, int ACT>
-__global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_sums_kernel(const __grid_constant__ GnArgs a) {
+template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_sums_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kUnrollB;
-    __shared__ __align__(16) F2 red[P * kThreads];
-    __shared__ __align__(16) F2 tot[2 * P * kMaxCols];
+    __shared__ __align__(16) F2 red[PLANES ? kWarps : P * kThreads];
+    __shared__ __align__(16) F2 tot[PLANES ? 1 : 2 * P * kMaxCols];
     extern __shared__ __align__(16) unsigned char gn_smem[];
     float4 *st = reinterpret_cast<float4 *>(gn_smem + BackwardFeed::bytes);
     float2 *acc = reinterpret_cast<float2 *>(st + a.gu);
@@ -952,19 +950,20 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_sums_kernel(const 
     const uint4 *xv = reinterpret_cast<const uint4 *>(x + k.head), *dv = reinterpret_cast<const uint4 *>(dy + k.head);
     float2 *out = a.bpart + ((long long)k.unit * a.chunks + k.chunk) * a.cu;
     wait_for_previous();
+    let_next_begin();
     load_stats(a, k, st);
-    if (a.cu > 1)
+    if (!PLANES)
         for (int c = threadIdx.x; c < a.cu; c += kThreads) acc[c] = make_float2(0.f, 0.f);
     __syncthreads();
-    for (int win = 0; win < a.windows; ++win) {
-        const Share s = make_share<T>(a, k, win);
+    for (int win = 0; win < (PLANES ? 1 : a.windows); ++win) {
+        const Share s = make_share<T, PLANES>(a, k, win);
         BackwardFeed feed;
         feed.start(gn_smem, xv + s.first, dv + s.first, s.count, s.step);
         F2 q[2 * P], m[P], sc[P], sh[P];  // q: sum g, sum g (x - m)
         {
             float w[V], b[V];
             int g[V];
-            slot_params<V>(a, k, s.ch0, w, b, g);
+            slot_params<V, PLANES>(a, k, s.ch0, w, b, g);
 #pragma unroll
             for (int p = 0; p < P; ++p) {
                 const float4 u = st[g[2 * p]], v = st[g[2 * p + 1]];
@@ -997,7 +996,7 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_sums_kernel(const 
             one(rx[0], rd[0]);
             if (j + 1 < s.count) one(rx[1], rd[1]);
         }
-        if (a.cu == 1) {
+        if constexpr (PLANES) {
             float v[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -1026,9 +1025,7 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_sums_kernel(const 
                 }
                 out[0] = make_float2(t.x, st[0].z * fmaf(-st[0].y, t.x, t.y));  // sum g (x - m) -> sum g xh
             }
-            let_next_begin();
-            return;
-        }
+        } else {
         column_sums<2, P>(a, s, q, red, tot);
         const int period = a.cols * V, lo = win * a.win_cols * V, hi = min(lo + a.win_cols * V, period), shift = k.head % a.cu;
         for (int c = threadIdx.x; c < a.cu; c += kThreads) {
@@ -1056,8 +1053,8 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_sums_kernel(const 
             }
         }
         if (a.windows > 1) __syncthreads();
+        }
     }
-    let_next_begin();
 }
 
 // (sum h, sum h xh) of the groups of a chunk's unit
@@ -1179,29 +1176,29 @@ __device__ __forceinline__ void parameter_gradients(const GnArgs &a, int block) 
 __device__ __forceinline__ float2 group_terms(const float4 &v, const float2 &t) { return make_float2(-v.z * fmaf(-v.y * v.z, t.y, t.x) * v.w, -v.z * v.z * t.y * v.w); }
 
 // The last CTAs of the grid compute the parameters' gradients.
-template <typename T, int ACT>
-__global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_dx_kernel(const __grid_constant__ GnArgs a) {
+template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_dx_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kUnrollB;
-    extern __shared__ __align__(16) unsigned char gn_smem[];
-    float4 *st = reinterpret_cast<float4 *>(gn_smem + BackwardFeed::bytes);
-    float2 *gsum = reinterpret_cast<float2 *>(st + a.gu);
     const int tasks = a.out ? a.tasks2 : 0;
     if ((int)blockIdx.x >= tasks) {
         wait_for_previous();
-        parameter_gradients(a, blockIdx.x - tasks);
+        parameter_gradients(a, (int)blockIdx.x - tasks);
         return;
     }
+    extern __shared__ __align__(16) unsigned char gn_smem[];
+    float4 *st = reinterpret_cast<float4 *>(gn_smem + BackwardFeed::bytes);
+    float2 *gsum = reinterpret_cast<float2 *>(st + a.gu);
     const Chunk k = make_chunk<T>(a, tasks - 1 - (int)blockIdx.x, a.chunks2, a.chunk_px2);
     const T *x = reinterpret_cast<const T *>(a.x) + k.base, *dy = reinterpret_cast<const T *>(a.dy) + k.base;
     T *dx = reinterpret_cast<T *>(a.out) + k.base;
     const uint4 *xv = reinterpret_cast<const uint4 *>(x + k.head), *dv = reinterpret_cast<const uint4 *>(dy + k.head);
     uint4 *ov = reinterpret_cast<uint4 *>(dx + k.head);
-    for (int win = 0; win < a.windows; ++win) {
-        const Share s = make_share<T>(a, k, win);
+    for (int win = 0; win < (PLANES ? 1 : a.windows); ++win) {
+        const Share s = make_share<T, PLANES>(a, k, win);
         BackwardFeed feed;
         feed.start(gn_smem, xv + s.first, dv + s.first, s.count, s.step);  // (x and dy were complete before the sums)
         if (win == 0) {
             wait_for_previous();
+            let_next_begin();
             load_stats(a, k, st);
             group_sums(a, k, gsum);
             __syncthreads();
@@ -1210,7 +1207,7 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_dx_kernel(const __
         {
             float w[V], b[V];
             int g[V];
-            slot_params<V>(a, k, s.ch0, w, b, g);
+            slot_params<V, PLANES>(a, k, s.ch0, w, b, g);
 #pragma unroll
             for (int p = 0; p < P; ++p) {
                 const float4 u = st[g[2 * p]], v = st[g[2 * p + 1]];
@@ -1385,29 +1382,29 @@ int launch(const void *kernel, int grid, size_t smem, const GnArgs &a, cudaStrea
     return SHTB200_OK;
 }
 
-template <typename T, template <typename, int> class K> const void *by_activation(int act) {
-    switch (act) {
-        case SHTB200_ACT_RELU: return K<T, SHTB200_ACT_RELU>::get();
-        case SHTB200_ACT_SILU: return K<T, SHTB200_ACT_SILU>::get();
-        case SHTB200_ACT_GELU: return K<T, SHTB200_ACT_GELU>::get();
-        default: return K<T, SHTB200_ACT_NONE>::get();
+// the kernel of a descriptor's type, activation and layout
+enum Which { kStats, kApply, kSums, kDx };
+template <typename T, int ACT, bool PLANES> const void *kernel_of(Which w) {
+    switch (w) {
+        case kStats: return (const void *)gn_stats_kernel<T, PLANES>;
+        case kApply: return (const void *)gn_apply_kernel<T, ACT, PLANES>;
+        case kSums: return (const void *)gn_sums_kernel<T, ACT, PLANES>;
+        default: return (const void *)gn_dx_kernel<T, ACT, PLANES>;
     }
 }
-template <template <typename, int> class K> const void *kernel_for(const GroupNormDesc &d) {
-    return d.dtype == SHTB200_F32 ? by_activation<float, K>(d.activation) : d.dtype == SHTB200_BF16 ? by_activation<__nv_bfloat16, K>(d.activation) : by_activation<__half, K>(d.activation);
+template <typename T, int ACT> const void *kernel_of(Which w, bool planes) { return planes ? kernel_of<T, ACT, true>(w) : kernel_of<T, ACT, false>(w); }
+template <typename T> const void *kernel_of(Which w, bool planes, int act) {
+    switch (act) {
+        case SHTB200_ACT_RELU: return kernel_of<T, SHTB200_ACT_RELU>(w, planes);
+        case SHTB200_ACT_SILU: return kernel_of<T, SHTB200_ACT_SILU>(w, planes);
+        case SHTB200_ACT_GELU: return kernel_of<T, SHTB200_ACT_GELU>(w, planes);
+        default: return kernel_of<T, SHTB200_ACT_NONE>(w, planes);
+    }
 }
-template <typename T, int> struct Stats {
-    static const void *get() { return (const void *)gn_stats_kernel<T>; }
-};
-template <typename T, int ACT> struct Apply {
-    static const void *get() { return (const void *)gn_apply_kernel<T, ACT>; }
-};
-template <typename T, int ACT> struct SumsOf {
-    static const void *get() { return (const void *)gn_sums_kernel<T, ACT>; }
-};
-template <typename T, int ACT> struct Dx {
-    static const void *get() { return (const void *)gn_dx_kernel<T, ACT>; }
-};
+const void *kernel_of(Which w, const GroupNormDesc &d, const GnArgs &a) {
+    const bool planes = a.cu == 1;
+    return d.dtype == SHTB200_F32 ? kernel_of<float>(w, planes, d.activation) : d.dtype == SHTB200_BF16 ? kernel_of<__nv_bfloat16>(w, planes, d.activation) : kernel_of<__half>(w, planes, d.activation);
+}
 
 int check_desc(const GroupNormDesc *d) {
     if (!d) return fail(SHTB200_EINVAL, "group norm descriptor is null");
@@ -1459,9 +1456,9 @@ int group_norm_forward(const GroupNormDesc *d, const void *x, const float *lat, 
     a.bias = bias;
     a.stats = reinterpret_cast<float4 *>(stats);
     a.part = reinterpret_cast<float4 *>(ws);
-    if ((rc = launch(kernel_for<Stats>(*d), a.tasks, StatsFeed::bytes + (a.cu > 1 ? sizeof(Moments) * a.gu : 0), a, st))) return rc;
+    if ((rc = launch(kernel_of(kStats, *d, a), a.tasks, StatsFeed::bytes + (a.cu > 1 ? sizeof(Moments) * a.gu : 0), a, st))) return rc;
     if (!a.direct && (rc = launch((const void *)gn_finish_stats_kernel, a.B * a.G, 0, a, st))) return rc;
-    return launch(kernel_for<Apply>(*d), a.tasks2, ApplyFeed::bytes + sizeof(float4) * a.gu, a, st);
+    return launch(kernel_of(kApply, *d, a), a.tasks2, ApplyFeed::bytes + sizeof(float4) * a.gu, a, st);
 }
 
 int group_norm_backward(const GroupNormDesc *d, const void *dy, const void *x, const float *lat, const void *weight, const void *bias, const void *stats, void *dx, void *dweight,
@@ -1488,9 +1485,9 @@ int group_norm_backward(const GroupNormDesc *d, const void *dy, const void *x, c
     const int grads = dweight || dbias ? ceil_div(a.C, kWarps) : 0;
     if (!dx && !grads) return SHTB200_OK;
     const size_t smem = BackwardFeed::bytes + sizeof(float4) * a.gu + sizeof(float2) * std::max(a.cu, a.gu);
-    if ((rc = launch(kernel_for<SumsOf>(*d), a.tasks, smem, a, st))) return rc;
+    if ((rc = launch(kernel_of(kSums, *d, a), a.tasks, smem, a, st))) return rc;
     if (!a.direct && (rc = launch((const void *)gn_finish_sums_kernel, a.B * ceil_div(a.C, kFinishChannels), 0, a, st))) return rc;
-    return launch(kernel_for<Dx>(*d), (dx ? a.tasks2 : 0) + grads, smem, a, st);
+    return launch(kernel_of(kDx, *d, a), (dx ? a.tasks2 : 0) + grads, smem, a, st);
 }
 
 }  // namespace shtb200
