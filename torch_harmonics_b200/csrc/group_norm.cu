@@ -267,7 +267,7 @@ struct GnArgs {
     float eps;
     int cu, gu, cgu;   // channels, groups of a unit, channels of a group inside a unit: (C, G, cg) channels last, (1, 1, 1) for planes
     int chunks, chunk_px, tasks;  // of a unit for the sums; chunks of all units
-    int chunks2, chunk_px2, tasks2;  // the same for the second pass
+    int pieces, piece_px;         // of a chunk, for the second pass
     int cols, dup;                // lcm(cu, V) / V: vectors after which the channels repeat; how often each occurs in them
     int win_cols, windows, reps;  // columns a CTA covers at a time, how many windows that takes, vectors of a column it takes side by side
     int step_px, step_rows, step_cols;  // from a thread's vector to its next, in pixels, and as rows and columns of the grid
@@ -282,20 +282,29 @@ struct Chunk {
     int px0;         // its pixel
     int n, head, vecs;
 };
-template <typename T> __device__ __forceinline__ Chunk make_chunk(const GnArgs &a, int task, int chunks, int chunk_px) {
+// Piece `piece` of chunk `task`, pieces of `piece_px` pixels (the whole chunk: piece 0 of chunk_px); n <= 0 where a chunk has fewer.
+template <typename T> __device__ __forceinline__ Chunk make_chunk(const GnArgs &a, int task, int piece, int piece_px) {
     Chunk k;
-    k.unit = (int)((unsigned)task / (unsigned)chunks);
-    k.chunk = task - k.unit * chunks;
+    k.unit = (int)((unsigned)task / (unsigned)a.chunks);
+    k.chunk = task - k.unit * a.chunks;
     k.b = a.cl ? k.unit : (int)((unsigned)k.unit / (unsigned)a.C);
     k.c = a.cl ? 0 : k.unit - k.b * a.C;
-    k.px0 = k.chunk * chunk_px;
-    const int px = (int)min((long long)chunk_px, a.hw - k.px0);
+    const int in = piece * piece_px;
+    k.px0 = k.chunk * a.chunk_px + in;
+    const int px = (int)min((long long)min(piece_px, a.chunk_px - in), a.hw - k.px0);
     k.base = ((long long)k.unit * a.hw + k.px0) * a.cu;
     k.n = px * a.cu;
     const unsigned mis = (unsigned)((uintptr_t)(reinterpret_cast<const T *>(a.x) + k.base) & 15u);
     k.head = min(k.n, (int)(((16u - mis) & 15u) / (unsigned)sizeof(T)));
     k.vecs = (k.n - k.head) / kV<T>;
     return k;
+}
+
+// The second pass takes the last pieces of all chunks first, then the ones before: the sums have read their chunks side by side, so that is what L2
+// holds.
+template <typename T> __device__ __forceinline__ Chunk second_pass_chunk(const GnArgs &a, int block) {
+    const int back = (int)((unsigned)block / (unsigned)a.tasks);
+    return make_chunk<T>(a, block - back * a.tasks, a.pieces - 1 - back, a.piece_px);
 }
 
 // A thread's share of a window of a chunk: vectors first, first + step, ... (count of them); the channel (of the unit) of slot 0.
@@ -598,7 +607,7 @@ template <typename T, bool PLANES> __global__ void __launch_bounds__(kThreads, k
     F2(*extra)[kThreads] = reinterpret_cast<F2(*)[kThreads]>(red);
     extern __shared__ __align__(16) unsigned char gn_smem[];
     Moments *acc = reinterpret_cast<Moments *>(gn_smem + StatsFeed::bytes);
-    const Chunk k = make_chunk<T>(a, blockIdx.x, a.chunks, a.chunk_px);
+    const Chunk k = make_chunk<T>(a, blockIdx.x, 0, a.chunk_px);
     const T *x = reinterpret_cast<const T *>(a.x) + k.base;
     const uint4 *xv = reinterpret_cast<const uint4 *>(x + k.head);
     float4 *out = a.part + ((long long)k.unit * a.chunks + k.chunk) * a.gu;
@@ -802,7 +811,7 @@ __device__ __forceinline__ void unit_stats(const GnArgs &a, const Chunk &k, floa
             m.gather(p, n, stride, lane, 32);
             if (lane == 0) {
                 st[i] = m.stats(a);
-                if (k.chunk == 0 && (a.cl || k.c == g0 * a.cg)) a.stats[k.b * a.G + g0 + i] = st[i];
+                if (k.px0 == 0 && (a.cl || k.c == g0 * a.cg)) a.stats[k.b * a.G + g0 + i] = st[i];
             }
         }
     } else {
@@ -849,7 +858,8 @@ template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kT
     constexpr int V = kV<T>, P = kP<T>, U = kApplyUnroll;
     extern __shared__ __align__(16) unsigned char gn_smem[];
     float4 *st = reinterpret_cast<float4 *>(gn_smem + ApplyFeed::bytes);
-    const Chunk k = make_chunk<T>(a, a.tasks2 - 1 - (int)blockIdx.x, a.chunks2, a.chunk_px2);
+    const Chunk k = second_pass_chunk<T>(a, blockIdx.x);
+    if (k.n <= 0) return;
     const T *x = reinterpret_cast<const T *>(a.x) + k.base;
     T *y = reinterpret_cast<T *>(a.out) + k.base;
     const uint4 *xv = reinterpret_cast<const uint4 *>(x + k.head);
@@ -945,7 +955,7 @@ template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kT
     extern __shared__ __align__(16) unsigned char gn_smem[];
     float4 *st = reinterpret_cast<float4 *>(gn_smem + BackwardFeed::bytes);
     float2 *acc = reinterpret_cast<float2 *>(st + a.gu);
-    const Chunk k = make_chunk<T>(a, blockIdx.x, a.chunks, a.chunk_px);
+    const Chunk k = make_chunk<T>(a, blockIdx.x, 0, a.chunk_px);
     const T *x = reinterpret_cast<const T *>(a.x) + k.base, *dy = reinterpret_cast<const T *>(a.dy) + k.base;
     const uint4 *xv = reinterpret_cast<const uint4 *>(x + k.head), *dv = reinterpret_cast<const uint4 *>(dy + k.head);
     float2 *out = a.bpart + ((long long)k.unit * a.chunks + k.chunk) * a.cu;
@@ -1178,7 +1188,7 @@ __device__ __forceinline__ float2 group_terms(const float4 &v, const float2 &t) 
 // The last CTAs of the grid compute the parameters' gradients.
 template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_dx_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kUnrollB;
-    const int tasks = a.out ? a.tasks2 : 0;
+    const int tasks = a.out ? a.tasks * a.pieces : 0;
     if ((int)blockIdx.x >= tasks) {
         wait_for_previous();
         parameter_gradients(a, (int)blockIdx.x - tasks);
@@ -1187,7 +1197,8 @@ template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kT
     extern __shared__ __align__(16) unsigned char gn_smem[];
     float4 *st = reinterpret_cast<float4 *>(gn_smem + BackwardFeed::bytes);
     float2 *gsum = reinterpret_cast<float2 *>(st + a.gu);
-    const Chunk k = make_chunk<T>(a, tasks - 1 - (int)blockIdx.x, a.chunks2, a.chunk_px2);
+    const Chunk k = second_pass_chunk<T>(a, blockIdx.x);
+    if (k.n <= 0) return;
     const T *x = reinterpret_cast<const T *>(a.x) + k.base, *dy = reinterpret_cast<const T *>(a.dy) + k.base;
     T *dx = reinterpret_cast<T *>(a.out) + k.base;
     const uint4 *xv = reinterpret_cast<const uint4 *>(x + k.head), *dv = reinterpret_cast<const uint4 *>(dy + k.head);
@@ -1313,19 +1324,8 @@ struct Launch {
     size_t total() const { return part + csum; }
 };
 
-constexpr int kSumWaves = 1, kPassWaves = 2;
-
-// Chunks of a unit: `per_sm` CTAs for each of 148 SMs, but no chunk under 16 KB (what a CTA does besides costs some microseconds, which the
-// others on its SM have to cover).
-void cut(const GnArgs &a, int V, int per_sm, int *chunks, int *chunk_px, int *tasks) {
-    const int units = a.cl ? a.B : a.B * a.C;
-    const long long unit_vecs = a.hw * a.cu / V, most = std::max<long long>(1, std::min<long long>(a.hw, unit_vecs / (kThreads * 4)));
-    const long long n = std::min<long long>(most, std::max(1, per_sm * 148 / units));
-    *chunk_px = (int)((a.hw + n - 1) / n);
-    if (*chunk_px >= 256) *chunk_px = (*chunk_px + 31) / 32 * 32;  // (chunks of an aligned field begin aligned)
-    *chunks = (int)((a.hw + *chunk_px - 1) / *chunk_px);
-    *tasks = units * *chunks;
-}
+constexpr long long kPieceBytes = 128 << 10;
+constexpr int kMaxPieces = 4;
 
 Launch geometry(const GroupNormDesc &d, bool backward) {
     Launch l;
@@ -1356,8 +1356,19 @@ Launch geometry(const GroupNormDesc &d, bool backward) {
     a.step_px = (int)step_px;
     a.step_rows = (int)(step_px / a.nlon);
     a.step_cols = (int)(step_px % a.nlon);
-    cut(a, V, (backward ? kBackwardCtas : V == 4 ? kStatsCtas<float> : kStatsCtas<__half>) * kSumWaves, &a.chunks, &a.chunk_px, &a.tasks);
-    cut(a, V, (backward ? kBackwardCtas : kApplyCtas) * kPassWaves, &a.chunks2, &a.chunk_px2, &a.tasks2);
+    // Chunks for the sums: one for every CTA that 148 SMs hold, but none under 16 KB (what a CTA does besides costs some microseconds, which
+    // the others on its SM have to cover).
+    const int units = a.cl ? a.B : a.B * a.C, ctas = 148 * (backward ? kBackwardCtas : V == 4 ? kStatsCtas<float> : kStatsCtas<__half>);
+    const long long unit_vecs = a.hw * a.cu / V, most = std::max<long long>(1, std::min<long long>(a.hw, unit_vecs / (kThreads * 4)));
+    const long long n = std::min<long long>(most, std::max(1, ctas / units));
+    a.chunk_px = (int)((a.hw + n - 1) / n);
+    if (a.chunk_px >= 256) a.chunk_px = (a.chunk_px + 31) / 32 * 32;  // (chunks of an aligned field begin aligned)
+    a.chunks = (int)((a.hw + a.chunk_px - 1) / a.chunk_px);
+    a.tasks = units * a.chunks;
+    // pieces of them for the second pass
+    a.pieces = (int)std::max<long long>(1, std::min<long long>(kMaxPieces, (long long)a.chunk_px * a.cu * value_bytes(d.dtype) / kPieceBytes));
+    a.piece_px = ceil_div(a.chunk_px, a.pieces);
+    if (a.piece_px >= 256) a.piece_px = (a.piece_px + 31) / 32 * 32;
     a.direct = a.gu <= kWarps && (long long)a.chunks * (backward || !a.cl ? a.cg : 1) <= kDirect;
     l.part = up256((size_t)a.tasks * (backward ? a.cu * sizeof(float2) : a.gu * sizeof(float4)));
     if (backward && !a.direct) l.csum = up256((size_t)a.B * a.C * sizeof(double2));
@@ -1425,7 +1436,7 @@ int plan(const GroupNormDesc *d, bool backward, const void *ws, size_t ws_bytes,
     if (!ws || ws_bytes < l->total()) return fail(SHTB200_EWORKSPACE, "workspace too small: need " + std::to_string(l->total()) + " bytes");
     if (((uintptr_t)ws & 255) != 0) return fail(SHTB200_EINVAL, "workspace must be 256-byte aligned");
     if (((uintptr_t)stats & 15) != 0) return fail(SHTB200_EINVAL, "the statistics must be 16-byte aligned");
-    if ((long long)std::max(l->a.chunk_px, l->a.chunk_px2) * l->a.cu > (1 << 30)) return fail(SHTB200_EINVAL, "group norm shape too large");
+    if ((long long)l->a.chunk_px * l->a.cu > (1 << 30) || (long long)l->a.tasks * l->a.pieces > (1 << 30)) return fail(SHTB200_EINVAL, "group norm shape too large");
     return SHTB200_OK;
 }
 // vectors are aligned in all tensors or in none
@@ -1458,7 +1469,7 @@ int group_norm_forward(const GroupNormDesc *d, const void *x, const float *lat, 
     a.part = reinterpret_cast<float4 *>(ws);
     if ((rc = launch(kernel_of(kStats, *d, a), a.tasks, StatsFeed::bytes + (a.cu > 1 ? sizeof(Moments) * a.gu : 0), a, st))) return rc;
     if (!a.direct && (rc = launch((const void *)gn_finish_stats_kernel, a.B * a.G, 0, a, st))) return rc;
-    return launch(kernel_of(kApply, *d, a), a.tasks2, ApplyFeed::bytes + sizeof(float4) * a.gu, a, st);
+    return launch(kernel_of(kApply, *d, a), a.tasks * a.pieces, ApplyFeed::bytes + sizeof(float4) * a.gu, a, st);
 }
 
 int group_norm_backward(const GroupNormDesc *d, const void *dy, const void *x, const float *lat, const void *weight, const void *bias, const void *stats, void *dx, void *dweight,
@@ -1487,7 +1498,7 @@ int group_norm_backward(const GroupNormDesc *d, const void *dy, const void *x, c
     const size_t smem = BackwardFeed::bytes + sizeof(float4) * a.gu + sizeof(float2) * std::max(a.cu, a.gu);
     if ((rc = launch(kernel_of(kSums, *d, a), a.tasks, smem, a, st))) return rc;
     if (!a.direct && (rc = launch((const void *)gn_finish_sums_kernel, a.B * ceil_div(a.C, kFinishChannels), 0, a, st))) return rc;
-    return launch(kernel_of(kDx, *d, a), (dx ? a.tasks2 : 0) + grads, smem, a, st);
+    return launch(kernel_of(kDx, *d, a), (dx ? a.tasks * a.pieces : 0) + grads, smem, a, st);
 }
 
 }  // namespace shtb200
