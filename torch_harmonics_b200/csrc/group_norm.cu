@@ -23,6 +23,8 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <map>
+#include <mutex>
 #include <numeric>
 
 namespace shtb200 {
@@ -1375,9 +1377,24 @@ Launch geometry(const GroupNormDesc &d, bool backward) {
     return l;
 }
 
+// Once for every kernel and device (and size, where it grows): dynamic shared memory beyond the default.
+int allow_smem(const void *kernel, size_t smem) {
+    static std::mutex mutex;
+    static std::map<std::pair<const void *, int>, size_t> allowed;
+    int dev = 0;
+    SHT_CUDA_CHECK(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lock(mutex);
+    size_t &have = allowed[{kernel, dev}];
+    if (have >= smem) return SHTB200_OK;
+    SHT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    have = smem;
+    return SHTB200_OK;
+}
+
 // A launch that may begin while the one before it ends (the kernels wait for its results themselves).
 int launch(const void *kernel, int grid, size_t smem, const GnArgs &a, cudaStream_t st) {
-    if (smem > (16 << 10)) SHT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    int rc = allow_smem(kernel, smem);
+    if (rc) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(kThreads);

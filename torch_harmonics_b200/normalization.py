@@ -35,7 +35,7 @@ def _aligned(t):
 
 def _run(module, x, weight, bias, keep):
     """y and (with ``keep``) what the backward pass needs, for a dense ``x``."""
-    desc, ws_bytes, _ = module._call(x)
+    desc, ws_bytes, _ = module._call(x, weight)
     batch, dev = x.shape[0], x.device
     y = torch.empty_like(x)
     stats_bytes = (16 * batch * module.num_groups + 255) // 256 * 256
@@ -46,7 +46,7 @@ def _run(module, x, weight, bias, keep):
     at = stats.data_ptr()
     with _lib.on_device(dev.index) as stream:
         rc = _lib.load().shtb200_group_norm_forward(
-            desc, x.data_ptr(), _ptr(module.lat_weights), _ptr(weight), _ptr(bias), y.data_ptr(), at, ws.data_ptr() if keep else at + stats_bytes, ws_bytes, stream
+            desc, x.data_ptr(), _ptr(module._buffers["lat_weights"]), _ptr(weight), _ptr(bias), y.data_ptr(), at, ws.data_ptr() if keep else at + stats_bytes, ws_bytes, stream
         )
     if rc != 0:
         _lib.check(rc, "shtb200_group_norm_forward")
@@ -57,32 +57,39 @@ class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, module):
         y, stats = _run(module, x, weight, bias, True)
-        ctx.save_for_backward(x, weight, bias, stats, module.lat_weights)
-        ctx.call = module._call(x)
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.call, ctx.lat = module._call(x, weight), module._buffers["lat_weights"]
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, stats, lat = ctx.saved_tensors
-        desc, _, ws_bytes = ctx.call
-        new = torch.empty_like if x.shape[0] else torch.zeros_like
-        need = ctx.needs_input_grad
-        dx = torch.empty_like(x) if need[0] else None
-        dw = new(weight) if need[1] else None
-        db = new(bias) if need[2] else None
-        if x.shape[0] == 0:
-            return dx, dw, db, None
-        # the gradient comes in any layout (an expanded scalar, for a sum): the kernel reads it in the layout of x
-        dy = _aligned(_lib.dense(dy) if not desc.channels_last else dy.resolve_neg().contiguous(memory_format=torch.channels_last))
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
-        with _lib.on_device(x.device.index) as stream:
-            rc = _lib.load().shtb200_group_norm_backward(
-                desc, dy.data_ptr(), x.data_ptr(), _ptr(lat), _ptr(weight), _ptr(bias), stats.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(), ws_bytes, stream
-            )
-        if rc != 0:
-            _lib.check(rc, "shtb200_group_norm_backward")
+        # (where no graph of the gradients is built, there is nothing to guard)
+        return _guarded_gradients(ctx, dy) if torch.is_grad_enabled() else _gradients(ctx, dy)
+
+
+def _gradients(ctx, dy):
+    x, weight, bias, stats = ctx.saved_tensors
+    desc, _, ws_bytes = ctx.call
+    new = torch.empty_like if x.shape[0] else torch.zeros_like
+    need = ctx.needs_input_grad
+    dx = torch.empty_like(x) if need[0] else None
+    dw = new(weight) if need[1] else None
+    db = new(bias) if need[2] else None
+    if x.shape[0] == 0:
         return dx, dw, db, None
+    # the gradient comes in any layout (an expanded scalar, for a sum): the kernel reads it in the layout of x
+    dy = _aligned(_lib.dense(dy) if not desc.channels_last else dy.resolve_neg().contiguous(memory_format=torch.channels_last))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+    with _lib.on_device(x.device.index) as stream:
+        rc = _lib.load().shtb200_group_norm_backward(
+            desc, dy.data_ptr(), x.data_ptr(), _ptr(ctx.lat), _ptr(weight), _ptr(bias), stats.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(), ws_bytes, stream
+        )
+    if rc != 0:
+        _lib.check(rc, "shtb200_group_norm_backward")
+    return dx, dw, db, None
+
+
+_guarded_gradients = once_differentiable(_gradients)
 
 
 class GroupNormS2(nn.Module):
@@ -161,9 +168,9 @@ class GroupNormS2(nn.Module):
         state = super().__getstate__() if hasattr(super(), "__getstate__") else self.__dict__
         return {**state, "_calls": {}}
 
-    def _call(self, x):
+    def _call(self, x, weight):
         """(descriptor, workspace bytes forward, backward) of a call on ``x``: shapes and types only."""
-        param = torch.float32 if self.weight is None else self.weight.dtype
+        param = torch.float32 if weight is None else weight.dtype
         cl = not x.is_contiguous()
         key = (x.shape[0], x.dtype, param, cl, self.eps, self.activation)
         call = self._calls.get(key)
@@ -192,8 +199,9 @@ class GroupNormS2(nn.Module):
                 raise RuntimeError(f"GroupNormS2: the input is on {x.device}, the parameters on {weight.device}")
             if weight.dtype not in _DTYPES or bias.dtype != weight.dtype:
                 raise TypeError(f"GroupNormS2: weight and bias must both be float32, bfloat16 or float16, got {weight.dtype} and {bias.dtype}")
-        elif self.lat_weights is not None and self.lat_weights.device != x.device:
-            raise RuntimeError(f"GroupNormS2: the input is on {x.device}, the latitude weights on {self.lat_weights.device}")
+        lat = self._buffers["lat_weights"]
+        if lat is not None and lat.device != x.device:
+            raise RuntimeError(f"GroupNormS2: the input is on {x.device}, the latitude weights on {lat.device}")
         if not (x.is_contiguous() or x.is_contiguous(memory_format=torch.channels_last)) or x.is_neg():
             x = _lib.dense(x)
         x = _aligned(x)
