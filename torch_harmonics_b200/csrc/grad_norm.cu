@@ -14,6 +14,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace shtb200 {
 
@@ -21,21 +22,22 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTensors = 896;         // tensors of one launch: the table has to fit into 32,764 bytes of kernel arguments
+constexpr int kFewTensors = 64;          // a small table for few: copying 30 KB of arguments twice a call costs more than scaling a small network
 constexpr int kUnitBytes = 32768;        // one unit of work: 8 vectors of 16 bytes a thread, all of them in flight before the first is used
 constexpr int kVectors = kUnitBytes / 16 / kThreads;
 constexpr int kScaleVectors = 4;         // (eight in flight spill: the scaling kernel also holds the addresses it writes to)
 constexpr int kBlocksPerSm = 4;
 constexpr int kMaxBlocks = 148 * kBlocksPerSm;
 
-struct Table {
-    const void *src[kMaxTensors];
-    void *dst[kMaxTensors];
-    long long n[kMaxTensors];            // values (a complex entry is two)
-    int first[kMaxTensors + 1];          // first unit of work of every tensor
-    unsigned char dtype[kMaxTensors];
-    int count = 0;
+template <int N> struct Table {
+    const void *src[N];
+    void *dst[N];
+    long long n[N];                      // values (a complex entry is two)
+    int first[N + 1];                    // first unit of work of every tensor
+    unsigned char dtype[N];
+    int count;
 };
-static_assert(sizeof(Table) + 64 <= 32764, "kernel arguments");
+static_assert(sizeof(Table<kMaxTensors>) + 64 <= 32764, "kernel arguments");
 
 __host__ __device__ constexpr int unit_values(int dtype) { return dtype == SHTB200_BF16 || dtype == SHTB200_F16 ? kUnitBytes / 2 : kUnitBytes / 4; }
 
@@ -77,7 +79,7 @@ template <> __device__ __forceinline__ void Pack<__half>::scale(float f) {
 }
 
 // Last tensor that starts at or before `unit`, searched from `lo` on (the units of a block ascend or descend).
-__device__ __forceinline__ int tensor_of(const Table &t, int unit, int lo, int hi) {
+template <int N> __device__ __forceinline__ int tensor_of(const Table<N> &t, int unit, int lo, int hi) {
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (t.first[mid] <= unit) lo = mid;
@@ -85,6 +87,10 @@ __device__ __forceinline__ int tensor_of(const Table &t, int unit, int lo, int h
     }
     return lo;
 }
+
+// The launches of a call may begin while the one before ends; each waits for its results (and so for all before) before it reads anything.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // (fmax drops a NaN; the largest magnitude has to keep it)
 __device__ __forceinline__ double larger(double a, double b) { return (b > a || b != b) ? b : a; }
@@ -138,8 +144,10 @@ __device__ __forceinline__ void gather_unit(const T *p, int n, bool pairs, doubl
 }
 
 // Partial sums of squares (or largest magnitudes, squared): one float64 value a block.
-template <int kind>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) norm_partial_kernel(const __grid_constant__ Table t, double *part) {
+template <int kind, int N>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) norm_partial_kernel(const __grid_constant__ Table<N> t, double *part) {
+    wait_for_previous();
+    let_next_begin();
     double acc[2] = {0., 0.}, pair[2] = {0., 0.};
     const int units = t.first[t.count];
     int k = 0;
@@ -167,6 +175,7 @@ template <int kind> __device__ float total_norm(const double *part, int nparts) 
 
 template <int kind>
 __global__ void __launch_bounds__(kThreads) norm_total_kernel(const double *part, int nparts, float *norm) {
+    wait_for_previous();
     const float v = total_norm<kind>(part, nparts);
     if (threadIdx.x == 0) *norm = v;
 }
@@ -204,8 +213,9 @@ __device__ __forceinline__ void scale_unit(const T *p, T *d, int n, float f) {
 }
 
 // The units are taken from the end: what the norm has read last is still in L2.
-template <int kind>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) scale_kernel(const __grid_constant__ Table t, const double *part, int nparts, float max_norm, float *norm) {
+template <int kind, int N>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) scale_kernel(const __grid_constant__ Table<N> t, const double *part, int nparts, float max_norm, float *norm) {
+    wait_for_previous();
     float total;
     if (part) {
         total = total_norm<kind>(part, nparts);
@@ -267,43 +277,82 @@ size_t grad_norm_workspace(int count) { return sizeof(double) * (size_t)kMaxBloc
 
 namespace {
 
-// The tables of a list of tensors, kMaxTensors a launch; empty tensors are left out.
-std::vector<Table> make_tables(int count, const void *const *src, void *const *dst, const long long *numel, const int *dtype) {
-    std::vector<Table> tables;
-    long long units = 0;
-    for (int i = 0; i < count; ++i) {
-        if (numel[i] == 0) continue;
-        const long long n = numel[i] * (dtype[i] == SHTB200_C64 ? 2 : 1), u = (n + unit_values(dtype[i]) - 1) / unit_values(dtype[i]);
-        if (tables.empty() || tables.back().count == kMaxTensors) {
-            tables.emplace_back();
-            units = 0;
+template <typename... P> int launch(void (*kernel)(P...), int grid, cudaStream_t st, std::remove_const_t<P> &...args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    void *pointers[] = {&args...};  // (the table is not copied on the way)
+    SHT_CUDA_CHECK(cudaLaunchKernelExC(&cfg, (const void *)kernel, pointers));
+    return SHTB200_OK;
+}
+
+// A list of tensors, kMaxTensors a launch; empty tensors are left out.
+struct List {
+    const void *const *src;
+    void *const *dst;
+    const long long *numel;
+    const int *dtype;
+    std::vector<int> index;  // of the tensors that are not empty
+    int launches() const { return ceil_div((int)index.size(), kMaxTensors); }
+    int count(int launch) const { return std::min(kMaxTensors, (int)index.size() - launch * kMaxTensors); }
+    template <int N> void fill(int launch, Table<N> *t) const {
+        t->count = count(launch);
+        t->first[0] = 0;
+        for (int k = 0; k < t->count; ++k) {
+            const int i = index[(size_t)launch * kMaxTensors + k];
+            t->src[k] = src[i];
+            t->dst[k] = dst ? dst[i] : nullptr;
+            t->n[k] = numel[i] * (dtype[i] == SHTB200_C64 ? 2 : 1);
+            t->dtype[k] = (unsigned char)dtype[i];
+            t->first[k + 1] = t->first[k] + (int)((t->n[k] + unit_values(dtype[i]) - 1) / unit_values(dtype[i]));
         }
-        Table &t = tables.back();
-        const int k = t.count++;
-        t.src[k] = src[i];
-        t.dst[k] = dst ? dst[i] : nullptr;
-        t.n[k] = n;
-        t.dtype[k] = (unsigned char)dtype[i];
-        t.first[k] = (int)units;
-        units += u;
-        t.first[k + 1] = (int)units;
     }
-    return tables;
+};
+List make_list(int count, const void *const *src, void *const *dst, const long long *numel, const int *dtype) {
+    List l{src, dst, numel, dtype, {}};
+    l.index.reserve((size_t)std::max(count, 0));
+    for (int i = 0; i < count; ++i)
+        if (numel[i]) l.index.push_back(i);
+    return l;
 }
 
-int blocks_of(const Table &t) { return std::min(kMaxBlocks, t.first[t.count]); }
-
-int launch_partials(const std::vector<Table> &tables, int kind, double *part, cudaStream_t st) {
-    int nparts = 0;
-    for (const Table &t : tables) {
-        (kind == SHTB200_NORM_INF ? norm_partial_kernel<SHTB200_NORM_INF> : norm_partial_kernel<SHTB200_NORM_L2>)<<<blocks_of(t), kThreads, 0, st>>>(t, part + nparts);
-        nparts += blocks_of(t);
-    }
-    return nparts;
+template <int N> int launch_partials(const List &l, int i, int kind, double *part, int *nparts, cudaStream_t st) {
+    Table<N> t;
+    l.fill(i, &t);
+    const int blocks = std::min(kMaxBlocks, t.first[t.count]);
+    double *to = part + *nparts;
+    const int rc = launch(kind == SHTB200_NORM_INF ? norm_partial_kernel<SHTB200_NORM_INF, N> : norm_partial_kernel<SHTB200_NORM_L2, N>, blocks, st, t, to);
+    *nparts += blocks;
+    return rc;
 }
-
-void launch_total(const double *part, int nparts, int kind, float *norm, cudaStream_t st) {
-    (kind == SHTB200_NORM_INF ? norm_total_kernel<SHTB200_NORM_INF> : norm_total_kernel<SHTB200_NORM_L2>)<<<1, kThreads, 0, st>>>(part, nparts, norm);
+int launch_partials(const List &l, int kind, double *part, int *nparts, cudaStream_t st) {
+    *nparts = 0;
+    int rc = SHTB200_OK;
+    for (int i = 0; i < l.launches() && !rc; ++i)
+        rc = l.count(i) <= kFewTensors ? launch_partials<kFewTensors>(l, i, kind, part, nparts, st) : launch_partials<kMaxTensors>(l, i, kind, part, nparts, st);
+    return rc;
+}
+template <int N> int launch_scale(const List &l, int i, int kind, const double *part, int nparts, float max_norm, float *norm, cudaStream_t st) {
+    Table<N> t;
+    l.fill(i, &t);
+    const int blocks = std::min(kMaxBlocks, t.first[t.count]);
+    return launch(kind == SHTB200_NORM_INF ? scale_kernel<SHTB200_NORM_INF, N> : scale_kernel<SHTB200_NORM_L2, N>, blocks, st, t, part, nparts, max_norm, norm);
+}
+int launch_scale(const List &l, int kind, const double *part, int nparts, float max_norm, float *norm, cudaStream_t st) {
+    int rc = SHTB200_OK;
+    for (int i = 0; i < l.launches() && !rc; ++i)
+        rc = l.count(i) <= kFewTensors ? launch_scale<kFewTensors>(l, i, kind, part, nparts, max_norm, norm, st)
+                                       : launch_scale<kMaxTensors>(l, i, kind, part, nparts, max_norm, norm, st);
+    return rc;
+}
+int launch_total(const double *part, int nparts, int kind, float *norm, cudaStream_t st) {
+    return launch(kind == SHTB200_NORM_INF ? norm_total_kernel<SHTB200_NORM_INF> : norm_total_kernel<SHTB200_NORM_L2>, 1, st, part, nparts, norm);
 }
 
 int check_norm(int count, int kind, const float *norm, const void *ws, size_t ws_bytes) {
@@ -319,12 +368,10 @@ int check_norm(int count, int kind, const float *norm, const void *ws, size_t ws
 int grad_norm(int count, const void *const *src, const long long *numel, const int *dtype, int kind, float *norm, void *ws, size_t ws_bytes, cudaStream_t st) {
     int rc = check_norm(count, kind, norm, ws, ws_bytes);
     if (rc || (rc = check_tensors(count, src, nullptr, numel, dtype))) return rc;
-    const std::vector<Table> tables = make_tables(count, src, nullptr, numel, dtype);
     double *part = reinterpret_cast<double *>(ws);
-    const int nparts = launch_partials(tables, kind, part, st);
-    launch_total(part, nparts, kind, norm, st);
-    SHT_CUDA_CHECK(cudaGetLastError());
-    return SHTB200_OK;
+    int nparts = 0;
+    if ((rc = launch_partials(make_list(count, src, nullptr, numel, dtype), kind, part, &nparts, st))) return rc;
+    return launch_total(part, nparts, kind, norm, st);
 }
 
 int clip_grads(int count, const void *const *src, void *const *dst, const long long *numel, const int *dtype, int kind, float max_norm, float *norm, void *ws, size_t ws_bytes,
@@ -332,14 +379,11 @@ int clip_grads(int count, const void *const *src, void *const *dst, const long l
     if (!(max_norm >= 0.f)) return fail(SHTB200_EINVAL, "max_norm must be >= 0");
     int rc = check_norm(count, kind, norm, ws, ws_bytes);
     if (rc || (rc = check_tensors(count, src, dst, numel, dtype))) return rc;
-    const std::vector<Table> tables = make_tables(count, src, dst, numel, dtype);
+    const List l = make_list(count, src, dst, numel, dtype);
     double *part = reinterpret_cast<double *>(ws);
-    const int nparts = launch_partials(tables, kind, part, st);
-    if (tables.empty()) launch_total(part, nparts, kind, norm, st);
-    for (const Table &t : tables)
-        (kind == SHTB200_NORM_INF ? scale_kernel<SHTB200_NORM_INF> : scale_kernel<SHTB200_NORM_L2>)<<<blocks_of(t), kThreads, 0, st>>>(t, part, nparts, max_norm, norm);
-    SHT_CUDA_CHECK(cudaGetLastError());
-    return SHTB200_OK;
+    int nparts = 0;
+    if ((rc = launch_partials(l, kind, part, &nparts, st))) return rc;
+    return l.index.empty() ? launch_total(part, nparts, kind, norm, st) : launch_scale(l, kind, part, nparts, max_norm, norm, st);
 }
 
 int scale_grads(int count, const void *const *src, void *const *dst, const long long *numel, const int *dtype, float max_norm, const float *norm, cudaStream_t st) {
@@ -347,9 +391,7 @@ int scale_grads(int count, const void *const *src, void *const *dst, const long 
     if (!norm) return fail(SHTB200_EINVAL, "null pointer");
     int rc = check_tensors(count, src, dst, numel, dtype);
     if (rc) return rc;
-    for (const Table &t : make_tables(count, src, dst, numel, dtype)) scale_kernel<SHTB200_NORM_L2><<<blocks_of(t), kThreads, 0, st>>>(t, nullptr, 0, max_norm, const_cast<float *>(norm));
-    SHT_CUDA_CHECK(cudaGetLastError());
-    return SHTB200_OK;
+    return launch_scale(make_list(count, src, dst, numel, dtype), SHTB200_NORM_L2, nullptr, 0, max_norm, const_cast<float *>(norm), st);
 }
 
 }  // namespace shtb200
