@@ -848,15 +848,15 @@ __global__ void __launch_bounds__(kThreads) gn_finish_stats_kernel(const __grid_
     let_next_begin();
 }
 
-constexpr int kApplyCtas = 4;  // on an SM
+template <typename T, bool PLANES> constexpr int kApplyCtas = sizeof(T) == 2 && !PLANES ? 3 : 4;  // on an SM (8 slots of different channels spill at 4)
 constexpr int kApplyUnroll = 2;
-using ApplyFeed = Feed<1, kApplyUnroll, 6>;
+using ApplyFeed = Feed<1, kApplyUnroll, 4>;
 
 // Scale and shift of a slot.  float32: z = (x - m) sc + sh, the difference first, so that a level far above the spread costs nothing.
 // 16-bit values carry that error many times over themselves: z = x sc + sh, m in the shift.
 template <typename T> constexpr bool kCentred = sizeof(T) == 4;
 
-template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kThreads, kApplyCtas) gn_apply_kernel(const __grid_constant__ GnArgs a) {
+template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kThreads, kApplyCtas<T, PLANES>) gn_apply_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kApplyUnroll;
     extern __shared__ __align__(16) unsigned char gn_smem[];
     float4 *st = reinterpret_cast<float4 *>(gn_smem + ApplyFeed::bytes);
@@ -935,7 +935,7 @@ template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kT
 // ------------------------------------------------------------------------------------------------
 constexpr int kUnrollB = 2;
 constexpr int kBackwardCtas = 2;  // on an SM: what a thread keeps of 8 slots and the activation's constants spills at 3 (361x720x256 bf16 164 us, at 2 139 us)
-using BackwardFeed = Feed<2, kUnrollB, 4>;
+using BackwardFeed = Feed<2, kUnrollB, 2>;  // (deeper was slower: 721x1440x73 bf16 154 us with 2 rounds, 168 with 4)
 
 __device__ __forceinline__ void load_stats(const GnArgs &a, const Chunk &k, float4 *st) {
     if (a.cl)
@@ -1368,7 +1368,7 @@ Launch geometry(const GroupNormDesc &d, bool backward) {
     a.chunks = (int)((a.hw + a.chunk_px - 1) / a.chunk_px);
     a.tasks = units * a.chunks;
     // pieces of them for the second pass
-    a.pieces = (int)std::max<long long>(1, std::min<long long>(kMaxPieces, (long long)a.chunk_px * a.cu * value_bytes(d.dtype) / kPieceBytes));
+    a.pieces = (int)std::max<long long>(1, std::min<long long>(kMaxPieces, (long long)a.chunk_px * a.cu * value_bytes(d.dtype) / (backward ? 2 * kPieceBytes : kPieceBytes)));
     a.piece_px = ceil_div(a.chunk_px, a.pieces);
     if (a.piece_px >= 256) a.piece_px = (a.piece_px + 31) / 32 * 32;
     a.direct = a.gu <= kWarps && (long long)a.chunks * (backward || !a.cl ? a.cg : 1) <= kDirect;
