@@ -116,6 +116,7 @@ def _step(m, x, dy):
 SHAPES = [
     (1, 1, 1, 2, 1), (2, 6, 3, 5, 7), (3, 5, 5, 9, 17), (1, 8, 4, 33, 64), (2, 73, 1, 17, 33), (2, 73, 73, 12, 24), (2, 64, 8, 16, 32), (1, 300, 4, 8, 9),
     (2, 520, 8, 6, 10), (1, 3, 1, 129, 257), (1, 1100, 100, 5, 8), (5, 24, 2, 31, 62), (1, 2, 1, 3, 1), (1, 2500, 5, 3, 4), (70, 2, 2, 4, 6), (1, 4, 4, 181, 360), (1, 32, 2, 91, 180),
+    (1, 4096, 4096, 3, 4), (1, 4096, 1, 2, 3), (2, 129, 43, 7, 9), (1, 1032, 8, 16, 31), (3, 64, 1, 24, 48),
 ]  # fmt: skip
 
 
@@ -450,3 +451,55 @@ def test_between_spectral_convolutions_in_training(fmt):
     opt.step()
     moved = math.sqrt(sum(float((p - b).abs().double().square().sum()) for p, b in zip(params, before)))
     assert abs(moved - 0.1 * 0.01) <= 1e-4 * 0.1 * 0.01 + 1e-7
+
+
+def _random_bf16(shape, seed):
+    x = torch.empty(shape, device="cuda", dtype=torch.bfloat16)
+    return x.normal_(generator=torch.Generator(device="cuda").manual_seed(seed))
+
+
+@pytest.mark.parametrize("fmt", ["planes", "last"])
+def test_more_values_than_32_bits_count(fmt):
+    """2,180,304,000 values: the last channels, behind 2^31, against a module of those channels alone (every channel its own group)."""
+    C, H, W, tail = 2100, 721, 1440, 3
+    if fmt == "planes":
+        x, dy = _random_bf16((1, C, H, W), 1), _random_bf16((1, C, H, W), 2)
+    else:
+        x, dy = (_random_bf16((1, H, W, C), i).permute(0, 3, 1, 2) for i in (1, 2))
+    m, small = _module(C, C, H, W, activation="silu"), _module(tail, tail, H, W, activation="silu")
+    with torch.no_grad():
+        m.weight.normal_(1, 0.3)
+        m.bias.normal_(0, 0.3)
+        small.weight.copy_(m.weight[-tail:])
+        small.bias.copy_(m.bias[-tail:])
+    y, dx, dw, db = _step(m, x, dy)
+    xs, dys = (t[:, -tail:].contiguous() for t in (x, dy))
+    _compare([y[:, -tail:], dx[:, -tail:], dw[-tail:], db[-tail:]], *_exact(small, xs, dys))
+    assert torch.isfinite(y[:, ::100]).all() and torch.isfinite(dw).all()
+
+
+def test_copies_after_use():
+    import copy
+    import pickle
+
+    m = _module(2, 6, 16, 32, activation="gelu")
+    x = torch.randn(1, 6, 16, 32, device="cuda")
+    want = m(x)
+    for n in (copy.deepcopy(m), pickle.loads(pickle.dumps(m))):
+        assert torch.equal(n(x), want)
+
+
+def test_inside_a_compiled_function():
+    """The surroundings may be compiled; the call itself runs as it is."""
+    m = _module(2, 6, 16, 32, activation="gelu")
+    _parameters(m)
+    x = torch.randn(2, 6, 16, 32, device="cuda", requires_grad=True)
+
+    def f(t):
+        return m(t * 2.0) + 1.0
+
+    want = f(x)
+    (g,) = torch.autograd.grad(want.square().sum(), x)
+    got = torch.compile(f, backend="aot_eager")(x)
+    (h,) = torch.autograd.grad(got.square().sum(), x)
+    assert torch.equal(got, want) and torch.equal(g, h)

@@ -42,7 +42,7 @@ def test_module_state():
 
 
 def test_construction_refusals():
-    for bad in (dict(num_groups=3, num_channels=4), dict(num_groups=0, num_channels=4), dict(num_groups=1, num_channels=0)):
+    for bad in (dict(num_groups=3, num_channels=4), dict(num_groups=0, num_channels=4), dict(num_groups=1, num_channels=0), dict(num_groups=1, num_channels=4097)):
         with pytest.raises(ValueError):
             th.GroupNormS2(**bad, img_shape=(13, 24))
     with pytest.raises(ValueError, match="Unknown activation"):
@@ -96,6 +96,15 @@ def test_c_abi_refuses_bad_descriptors(lib):
     assert lib.shtb200_group_norm_forward(d, None, None, None, None, fake, fake, fake, 1 << 30, None) == -1
     assert lib.shtb200_group_norm_forward(d, fake, None, None, None, fake, fake, fake, 8, None) == -3
     assert lib.shtb200_group_norm_forward(d, fake, None, None, None, fake, fake, None, 1 << 30, None) == -3
+    assert lib.shtb200_group_norm_forward(d, fake, None, None, None, fake + 4, fake, fake, 1 << 30, None) == -1 and b"modulo 16" in lib.shtb200_last_error()
+    assert lib.shtb200_group_norm_forward(d, fake, None, None, None, fake, fake + 8, fake, 1 << 30, None) == -1
+    assert lib.shtb200_group_norm_forward(d, fake, None, None, None, fake, fake, fake + 16, 1 << 30, None) == -1
+    assert lib.shtb200_group_norm_backward(d, fake + 4, fake, None, None, None, fake, fake, None, None, fake, 1 << 30, None) == -1
+    assert lib.shtb200_group_norm_backward(d, fake, fake, None, None, None, fake, fake + 2, None, None, fake, 1 << 30, None) == -1
+    assert lib.shtb200_group_norm_backward(_lib.GroupNormDesc(**{**good, "batch": 0}), fake, fake, None, None, None, fake, fake, None, None, fake, 1 << 30, None) == -1
+    # nothing to do: no device is touched
+    assert lib.shtb200_group_norm_forward(_lib.GroupNormDesc(**{**good, "batch": 0}), None, None, None, None, None, None, None, 0, None) == 0
+    assert lib.shtb200_group_norm_backward(d, fake, fake, None, None, None, fake, None, None, None, fake, 1 << 30, None) == 0
 
 
 def _lists(tensors):

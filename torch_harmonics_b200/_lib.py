@@ -21,6 +21,7 @@ ENGINES = {"auto": ENGINE_AUTO, "simt": ENGINE_SIMT, "tcgen05": ENGINE_TCGEN05}
 F32, BF16, F16, C64 = range(4)
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
 NORM_L2, NORM_INF = range(2)
+GROUP_NORM_MAX_CHANNELS = 4096
 
 
 class GroupNormDesc(ctypes.Structure):

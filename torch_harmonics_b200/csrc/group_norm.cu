@@ -1313,7 +1313,7 @@ template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kT
 // ------------------------------------------------------------------------------------------------
 // host
 // ------------------------------------------------------------------------------------------------
-constexpr int kMaxChannels = 4096;  // what a CTA keeps per channel or group has to fit into its shared memory
+constexpr int kMaxChannels = SHTB200_GROUP_NORM_MAX_CHANNELS;  // what a CTA keeps per channel or group has to fit into its shared memory
 constexpr int kDirect = 128;        // partial results of a group up to which every CTA joins them itself, a warp a group, instead of a launch in between
 
 int value_bytes(int dtype) { return dtype == SHTB200_F32 ? 4 : 2; }

@@ -129,6 +129,8 @@ class GroupNormS2(nn.Module):
             raise ValueError(f"num_groups ({num_groups}) and num_channels ({num_channels}) must be positive")
         if num_channels % num_groups != 0:
             raise ValueError(f"num_channels ({num_channels}) must be divisible by num_groups ({num_groups})")
+        if num_channels > _lib.GROUP_NORM_MAX_CHANNELS:
+            raise ValueError(f"num_channels ({num_channels}) must not exceed {_lib.GROUP_NORM_MAX_CHANNELS}")
         if activation not in _lib.ACTIVATIONS:
             raise ValueError(f"Unknown activation {activation!r}, expected one of {list(_lib.ACTIVATIONS)}")
         if not eps >= 0.0:
