@@ -356,10 +356,18 @@ __device__ __forceinline__ void advance(const GnArgs &a, Rows &r) {
     }
 }
 // weights of the slots of a vector across a row's end
-template <typename T> __device__ __noinline__ void mixed_weights(const float *lat, int nlon, int cu, int ch0, int row, int col, float *w) {
+template <typename T> __device__ __forceinline__ void mixed_weights(const float *lat, int nlon, int cu, int ch, int row, int col, float (&w)[kV<T>]) {
+#pragma unroll
     for (int i = 0; i < kV<T>; ++i) {
-        const int px = col + (ch0 + i) / cu;
-        w[i] = lat[row + px / nlon];
+        while (col >= nlon) {
+            col -= nlon;
+            ++row;
+        }
+        w[i] = __ldg(lat + row);
+        if (++ch == cu) {
+            ch = 0;
+            ++col;
+        }
     }
 }
 // value i of the head and tail of a chunk (fewer than 2 V values): its index in the chunk, -1 beyond
@@ -424,12 +432,19 @@ template <int V, bool PLANES> __device__ __forceinline__ void slot_params(const 
 // ------------------------------------------------------------------------------------------------
 // joining of moments
 // ------------------------------------------------------------------------------------------------
-struct Moments {  // (sum of weights, K, mean - K, M2)
+struct Moments {  // (sum of weights, K, mean - K, M2); K is the mean rounded: a K far out (the value at a pole) would round mean - K
     float W, K, m, M2;
 };
+__device__ __forceinline__ void normalise(Moments &a) {
+    const float K = a.K + a.m;
+    a.m = (a.K - K) + a.m;
+    a.K = K;
+}
 __device__ __forceinline__ Moments moments(float W, float c, float S1, float S2) {
     const float m = W > 0.f ? __fdividef(S1, W) : 0.f;
-    return {W, c, m, fmaxf(fmaf(-S1, m, S2), S2 * 0.f)};  // (rounding may leave less than nothing; a NaN or infinity has to stay)
+    Moments r{W, c, m, fmaxf(fmaf(-S1, m, S2), S2 * 0.f)};  // (rounding may leave less than nothing; a NaN or infinity has to stay)
+    normalise(r);
+    return r;
 }
 __device__ __forceinline__ void join(Moments &a, const Moments &b) {
     if (b.W == 0.f) return;
@@ -441,6 +456,7 @@ __device__ __forceinline__ void join(Moments &a, const Moments &b) {
     a.m = fmaf(d, f, a.m);
     a.M2 += fmaf(d * d, a.W * f, b.M2);
     a.W = W;
+    normalise(a);
 }
 
 __device__ __forceinline__ double warp_sum(double v) {
@@ -588,6 +604,10 @@ template <typename T> __device__ __forceinline__ void accumulate(const F2 (&v)[k
         q[kP<T> + p] = fma2(wd, d, q[kP<T> + p]);
     }
 }
+__device__ __forceinline__ F2 reciprocal(F2 a) {
+    const float2 v = split(a);
+    return f2(__fdividef(1.f, v.x), __fdividef(1.f, v.y));
+}
 // sums about c + delta from those about c
 __device__ __forceinline__ void recentre(F2 W, F2 delta, F2 &S1, F2 &S2) {
     const F2 t = mul2(W, delta);
@@ -688,11 +708,10 @@ template <typename T, bool PLANES> __global__ void __launch_bounds__(kThreads, k
                 }
                 const int round = j / U;
                 if ((round & (round + 1)) == 0) {
-                    const F2 inv = f2(__fdividef(1.f, W));
 #pragma unroll
                     for (int p = 0; p < P; ++p) {
-                        const F2 to = fma2(q[p], inv, c[p]), delta = sub2(to, c[p]);
-                        recentre(add2(f2(W), extra[p][threadIdx.x]), delta, q[p], q[P + p]);
+                        const F2 Wp = add2(extra[p][threadIdx.x], f2(W)), to = fma2(q[p], reciprocal(Wp), c[p]), delta = sub2(to, c[p]);
+                        recentre(Wp, delta, q[p], q[P + p]);
                         c[p] = to;
                     }
                 }
