@@ -11,7 +11,9 @@
 // work is cut into units (a sample, channels last; a plane, otherwise), units into chunks of pixels, a CTA each.  A chunk is read as one flat stream of
 // 16-byte vectors: with C' interleaved channels (C, or 1 for planes) and V values a vector, a thread that steps by a multiple of lcm(C', V)
 // values meets the same channels in every vector ("slots"), whatever C' is, and keeps their sums and parameters in registers.  The second
-// pass takes the chunks from the last one on: what the first has read last is still in L2.
+// pass takes the last pieces of all chunks first: what the first has read last is still in L2.
+//
+// All times below are device times on a B200 with a cold L2 (fields in HBM, copied at 6.56 TB/s).
 //
 // Sums for the variance are taken about a centre c per slot, (W, c, S1, S2) = (sum a, c, sum a (x - c), sum a (x - c)^2).  c begins as a value
 // of the field and is moved to the mean so far after 1, 2, 4, 8, ... rounds; fields whose level is far above their spread (pressures) or
@@ -323,13 +325,13 @@ template <typename T, bool PLANES> __device__ __forceinline__ Share make_share(c
         s.step = 32;
         s.count = s.first < hi ? (hi - s.first + 31) / 32 : 0;
     } else {
-    s.rep = a.win_cols == 1 ? (int)threadIdx.x : (int)(threadIdx.x / (unsigned)a.win_cols);
-    s.col = (int)threadIdx.x - s.rep * a.win_cols;
-    const int c = window * a.win_cols + s.col;
-    s.first = c + s.rep * a.cols;
-    s.step = a.reps * a.cols;
-    s.count = (s.rep < a.reps && c < a.cols && s.first < k.vecs) ? (int)((unsigned)(k.vecs - s.first + s.step - 1) / (unsigned)s.step) : 0;
-    s.ch0 = (int)((unsigned)(c * kV<T> + k.head) % (unsigned)a.cu);
+        s.rep = a.win_cols == 1 ? (int)threadIdx.x : (int)(threadIdx.x / (unsigned)a.win_cols);
+        s.col = (int)threadIdx.x - s.rep * a.win_cols;
+        const int c = window * a.win_cols + s.col;
+        s.first = c + s.rep * a.cols;
+        s.step = a.reps * a.cols;
+        s.count = (s.rep < a.reps && c < a.cols && s.first < k.vecs) ? (int)((unsigned)(k.vecs - s.first + s.step - 1) / (unsigned)s.step) : 0;
+        s.ch0 = (int)((unsigned)(c * kV<T> + k.head) % (unsigned)a.cu);
     }
     return s;
 }
@@ -616,8 +618,11 @@ __device__ __forceinline__ void recentre(F2 W, F2 delta, F2 &S1, F2 &S2) {
 }
 
 constexpr int kUnroll = 2;
-template <typename T> constexpr int kStatsCtas = sizeof(T) == 4 ? 4 : 3;  // on an SM: 8 slots a thread need more registers than 4
-using StatsFeed = Feed<1, kUnroll, 3>;
+template <typename T> constexpr int kStatsCtas = sizeof(T) == 4 ? 4 : 3;  // on an SM: 8 slots a thread spill at 4 (73 channels bf16 126 us, at 3 101); 4 slots do not
+using StatsFeed = Feed<1, kUnroll, 3>;  // (721x1440x73 bf16 channels last, forward: 101 us with 3 rounds, 103 with 2, 107 with 5)
+
+// Sums of a chunk.  Bound by reading x in float32; with 16-bit values by the instructions per value (convert, subtract, two sums in pairs).
+// 721x1440x73 float32 planes, with the pass below: 165 us, 5.5 TB/s over two reads and a write.
 
 template <typename T, bool PLANES> __global__ void __launch_bounds__(kThreads, kStatsCtas<T>) gn_stats_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kUnroll;
@@ -767,46 +772,46 @@ template <typename T, bool PLANES> __global__ void __launch_bounds__(kThreads, k
                 out[0] = make_float4(m.W, m.K, m.m, m.M2);
             }
         } else {
-        column_sums<3, P>(a, s, z, red, tot);
-        // groups: a few lanes each go through its channels' slots in this window
-        const int period = a.cols * V, slots = a.cgu * a.dup, shift = k.head % a.cu, L = a.lanes;
-        const int sub = threadIdx.x & (L - 1), lo = win * a.win_cols * V, hi = min(lo + a.win_cols * V, period);
-        for (int g0 = 0; g0 < a.gu; g0 += kThreads / L) {
-            const int g = g0 + (int)threadIdx.x / L;
-            Moments m{0.f, 0.f, 0.f, 0.f};
-            if (g < a.gu)
-                for (int i = sub; i < slots; i += L) {
-                    const int again = (int)((unsigned)i / (unsigned)a.cgu);
-                    int e = g * a.cgu + (i - again * a.cgu) - shift;  // value of the period that has this channel
-                    if (e < 0) e += a.cu;
-                    e += again * a.cu;
-                    if (e >= lo && e < hi) {
-                        const int col = (e - lo) / V, i2 = (e - lo) % V;
-                        join(m, moments(half_of(tot, i2 / 2, col, i2 & 1), centre[i2 * kMaxCols + col], half_of(tot, P + i2 / 2, col, i2 & 1), half_of(tot, 2 * P + i2 / 2, col, i2 & 1)));
+            column_sums<3, P>(a, s, z, red, tot);
+            // groups: a few lanes each go through its channels' slots in this window
+            const int period = a.cols * V, slots = a.cgu * a.dup, shift = k.head % a.cu, L = a.lanes;
+            const int sub = threadIdx.x & (L - 1), lo = win * a.win_cols * V, hi = min(lo + a.win_cols * V, period);
+            for (int g0 = 0; g0 < a.gu; g0 += kThreads / L) {
+                const int g = g0 + (int)threadIdx.x / L;
+                Moments m{0.f, 0.f, 0.f, 0.f};
+                if (g < a.gu)
+                    for (int i = sub; i < slots; i += L) {
+                        const int again = (int)((unsigned)i / (unsigned)a.cgu);
+                        int e = g * a.cgu + (i - again * a.cgu) - shift;  // value of the period that has this channel
+                        if (e < 0) e += a.cu;
+                        e += again * a.cu;
+                        if (e >= lo && e < hi) {
+                            const int col = (e - lo) / V, i2 = (e - lo) % V;
+                            join(m, moments(half_of(tot, i2 / 2, col, i2 & 1), centre[i2 * kMaxCols + col], half_of(tot, P + i2 / 2, col, i2 & 1), half_of(tot, 2 * P + i2 / 2, col, i2 & 1)));
+                        }
                     }
+                for (int o = L / 2; o; o >>= 1) {
+                    Moments b;
+                    b.W = __shfl_down_sync(0xffffffffu, m.W, o, L);
+                    b.K = __shfl_down_sync(0xffffffffu, m.K, o, L);
+                    b.m = __shfl_down_sync(0xffffffffu, m.m, o, L);
+                    b.M2 = __shfl_down_sync(0xffffffffu, m.M2, o, L);
+                    join(m, b);
                 }
-            for (int o = L / 2; o; o >>= 1) {
-                Moments b;
-                b.W = __shfl_down_sync(0xffffffffu, m.W, o, L);
-                b.K = __shfl_down_sync(0xffffffffu, m.K, o, L);
-                b.m = __shfl_down_sync(0xffffffffu, m.m, o, L);
-                b.M2 = __shfl_down_sync(0xffffffffu, m.M2, o, L);
-                join(m, b);
+                if (g < a.gu && sub == 0) {
+                    Moments t = acc[g];
+                    join(t, m);
+                    if (win == 0)  // the values outside the vectors, one at a time
+                        for (int i = 0; i < 2 * V; ++i) {
+                            const int e = ragged<T>(k, i);
+                            if (e < 0) break;
+                            if ((e % a.cu) / a.cgu == g) join(t, Moments{weight_at(a, k, e), to_f(x[e]), 0.f, 0.f});
+                        }
+                    acc[g] = t;
+                    if (win == a.windows - 1) out[g] = make_float4(t.W, t.K, t.m, t.M2);
+                }
             }
-            if (g < a.gu && sub == 0) {
-                Moments t = acc[g];
-                join(t, m);
-                if (win == 0)  // the values outside the vectors, one at a time
-                    for (int i = 0; i < 2 * V; ++i) {
-                        const int e = ragged<T>(k, i);
-                        if (e < 0) break;
-                        if ((e % a.cu) / a.cgu == g) join(t, Moments{weight_at(a, k, e), to_f(x[e]), 0.f, 0.f});
-                    }
-                acc[g] = t;
-                if (win == a.windows - 1) out[g] = make_float4(t.W, t.K, t.m, t.M2);
-            }
-        }
-        if (a.windows > 1) __syncthreads();
+            if (a.windows > 1) __syncthreads();
         }
     }
 }
@@ -867,14 +872,17 @@ __global__ void __launch_bounds__(kThreads) gn_finish_stats_kernel(const __grid_
     let_next_begin();
 }
 
-template <typename T, bool PLANES> constexpr int kApplyCtas = sizeof(T) == 2 && !PLANES ? 3 : 4;  // on an SM (8 slots of different channels spill at 4)
+template <typename T, bool PLANES> constexpr int kApplyCtas = sizeof(T) == 2 && !PLANES ? 3 : 4;  // on an SM: 8 slots of different channels keep
+// more parameters than 4 CTAs leave registers for (361x720x256 bf16 forward 91 us, at 3 87; float32 gains from 4: 16x128x256x32 42 us, at 3 44)
 constexpr int kApplyUnroll = 2;
-using ApplyFeed = Feed<1, kApplyUnroll, 4>;
+using ApplyFeed = Feed<1, kApplyUnroll, 4>;  // (721x1440x73 float32 forward: 165 us with 4 rounds, 169 with 2, 165 with 6)
 
 // Scale and shift of a slot.  float32: z = (x - m) sc + sh, the difference first, so that a level far above the spread costs nothing.
 // 16-bit values carry that error many times over themselves: z = x sc + sh, m in the shift.
 template <typename T> constexpr bool kCentred = sizeof(T) == 4;
 
+// y of a piece.  Bound by the write of y and the read of what L2 no longer holds of x; with 16-bit values and an activation by
+// its arithmetic too (721x1440x64 bf16 planes forward: 87 us with gelu and latitude weights, 73 without either).
 template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kThreads, kApplyCtas<T, PLANES>) gn_apply_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kApplyUnroll;
     extern __shared__ __align__(16) unsigned char gn_smem[];
@@ -953,8 +961,8 @@ template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kT
 // backward
 // ------------------------------------------------------------------------------------------------
 constexpr int kUnrollB = 2;
-constexpr int kBackwardCtas = 2;  // on an SM: what a thread keeps of 8 slots and the activation's constants spills at 3 (361x720x256 bf16 164 us, at 2 139 us)
-using BackwardFeed = Feed<2, kUnrollB, 2>;  // (deeper was slower: 721x1440x73 bf16 154 us with 2 rounds, 168 with 4)
+constexpr int kBackwardCtas = 2;  // on an SM: what a thread keeps of 8 slots and the activation's constants spills at 3 (361x720x256 bf16 153 us, at 2 134)
+using BackwardFeed = Feed<2, kUnrollB, 2>;  // (deeper was slower: 721x1440x73 bf16 155 us with 2 rounds, 163 with 3, 167 with 4)
 
 __device__ __forceinline__ void load_stats(const GnArgs &a, const Chunk &k, float4 *st) {
     if (a.cl)
@@ -969,6 +977,9 @@ template <typename T, int ACT> __device__ __forceinline__ float2 ragged_slope(co
     return make_float2(dy * split(act_slope<ACT, false>(f2(kSlopeScale<ACT> * fmaf(d, sc, sh)))).x, d);
 }
 
+// (sum g, sum g xh) of the channels of a chunk: the slope is evaluated here and again in the second pass, since storing g would cost a write and a
+// read of the field.  721x1440x64 float32 planes, with the pass below: 230 us, 5.8 TB/s over four reads and a write; 16-bit values are bound
+// by the slope's arithmetic (73 channels bf16: 155 us, 4.9 TB/s).
 template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_sums_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kUnrollB;
     __shared__ __align__(16) F2 red[PLANES ? kWarps : P * kThreads];
@@ -1057,33 +1068,33 @@ template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kT
                 out[0] = make_float2(t.x, st[0].z * fmaf(-st[0].y, t.x, t.y));  // sum g (x - m) -> sum g xh
             }
         } else {
-        column_sums<2, P>(a, s, q, red, tot);
-        const int period = a.cols * V, lo = win * a.win_cols * V, hi = min(lo + a.win_cols * V, period), shift = k.head % a.cu;
-        for (int c = threadIdx.x; c < a.cu; c += kThreads) {
-            float2 t = acc[c];
-            for (int e = c >= shift ? c - shift : c - shift + a.cu; e < hi; e += a.cu)
-                if (e >= lo) {
-                    const int col = (e - lo) / V, i = (e - lo) % V;
-                    t.x += half_of(tot, i / 2, col, i & 1);
-                    t.y += half_of(tot, P + i / 2, col, i & 1);
-                }
-            if (win == 0)
-                for (int i = 0; i < 2 * V; ++i) {
-                    const int e = ragged<T>(k, i);
-                    if (e < 0) break;
-                    if (e % a.cu == c) {
-                        const float2 g = ragged_slope<T, ACT>(a, k, st, to_f(x[e]), to_f(dy[e]), c);
-                        t.x += g.x;
-                        t.y = fmaf(g.x, g.y, t.y);
+            column_sums<2, P>(a, s, q, red, tot);
+            const int period = a.cols * V, lo = win * a.win_cols * V, hi = min(lo + a.win_cols * V, period), shift = k.head % a.cu;
+            for (int c = threadIdx.x; c < a.cu; c += kThreads) {
+                float2 t = acc[c];
+                for (int e = c >= shift ? c - shift : c - shift + a.cu; e < hi; e += a.cu)
+                    if (e >= lo) {
+                        const int col = (e - lo) / V, i = (e - lo) % V;
+                        t.x += half_of(tot, i / 2, col, i & 1);
+                        t.y += half_of(tot, P + i / 2, col, i & 1);
                     }
+                if (win == 0)
+                    for (int i = 0; i < 2 * V; ++i) {
+                        const int e = ragged<T>(k, i);
+                        if (e < 0) break;
+                        if (e % a.cu == c) {
+                            const float2 g = ragged_slope<T, ACT>(a, k, st, to_f(x[e]), to_f(dy[e]), c);
+                            t.x += g.x;
+                            t.y = fmaf(g.x, g.y, t.y);
+                        }
+                    }
+                acc[c] = t;
+                if (win == a.windows - 1) {
+                    const float4 v = st[c / a.cgu];
+                    out[c] = make_float2(t.x, v.z * fmaf(-v.y, t.x, t.y));
                 }
-            acc[c] = t;
-            if (win == a.windows - 1) {
-                const float4 v = st[c / a.cgu];
-                out[c] = make_float2(t.x, v.z * fmaf(-v.y, t.x, t.y));
             }
-        }
-        if (a.windows > 1) __syncthreads();
+            if (a.windows > 1) __syncthreads();
         }
     }
 }
@@ -1206,7 +1217,7 @@ __device__ __forceinline__ void parameter_gradients(const GnArgs &a, int block) 
 // dx = sc g - a (alpha + (x - m) beta),  alpha = r (sum h - lo r sum h xh) / sum a,  beta = r^2 sum h xh / sum a
 __device__ __forceinline__ float2 group_terms(const float4 &v, const float2 &t) { return make_float2(-v.z * fmaf(-v.y * v.z, t.y, t.x) * v.w, -v.z * v.z * t.y * v.w); }
 
-// The last CTAs of the grid compute the parameters' gradients.
+// dx of a piece.  The last CTAs of the grid compute the parameters' gradients: no launch of their own.
 template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_dx_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kUnrollB;
     const int tasks = a.out ? a.tasks * a.pieces : 0;
@@ -1333,7 +1344,9 @@ template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kT
 // host
 // ------------------------------------------------------------------------------------------------
 constexpr int kMaxChannels = SHTB200_GROUP_NORM_MAX_CHANNELS;  // what a CTA keeps per channel or group has to fit into its shared memory
-constexpr int kDirect = 128;        // partial results of a group up to which every CTA joins them itself, a warp a group, instead of a launch in between
+// Partial results of a group up to which every CTA joins them itself, a warp a group, instead of a launch in between.  (256x512x32 float32,
+// forward: 30 us with the launch, 42 without, which a limit of 512 would choose; 16x128x256x32: 42 us without, 44 with, which 32 would.)
+constexpr int kDirect = 128;
 
 int value_bytes(int dtype) { return dtype == SHTB200_F32 ? 4 : 2; }
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
@@ -1345,6 +1358,9 @@ struct Launch {
     size_t total() const { return part + csum; }
 };
 
+// Pieces of a chunk for the second pass: small ones follow what L2 holds more closely, large ones pay a CTA's start less often.  Forward, 721x1440x73
+// float32: 165 us, with whole chunks 172; 361x720x256 bf16: 87 us, with pieces of half the size 91 (backward, where they are twice as large:
+// 134 us, with half the size 142).
 constexpr long long kPieceBytes = 128 << 10;
 constexpr int kMaxPieces = 4;
 
@@ -1377,8 +1393,8 @@ Launch geometry(const GroupNormDesc &d, bool backward) {
     a.step_px = (int)step_px;
     a.step_rows = (int)(step_px / a.nlon);
     a.step_cols = (int)(step_px % a.nlon);
-    // Chunks for the sums: one for every CTA that 148 SMs hold, but none under 16 KB (what a CTA does besides costs some microseconds, which
-    // the others on its SM have to cover).
+    // Chunks for the sums: one for every CTA that 148 SMs hold, but none under 16 KB, what a CTA does besides costing some microseconds (128x256x32 bf16
+    // forward and backward: 17.4 us each, with 4 KB 19.5 each, with 64 KB 19.5 and 21.5).
     const int units = a.cl ? a.B : a.B * a.C, ctas = 148 * (backward ? kBackwardCtas : V == 4 ? kStatsCtas<float> : kStatsCtas<__half>);
     const long long unit_vecs = a.hw * a.cu / V, most = std::max<long long>(1, std::min<long long>(a.hw, unit_vecs / (kThreads * 4)));
     const long long n = std::min<long long>(most, std::max(1, ctas / units));
