@@ -503,3 +503,24 @@ def test_inside_a_compiled_function():
     got = torch.compile(f, backend="aot_eager")(x)
     (h,) = torch.autograd.grad(got.square().sum(), x)
     assert torch.equal(got, want) and torch.equal(g, h)
+
+
+def test_replaced_parameters():
+    """Parameters with strides, and one value expanded to all channels, whose gradient is the sum of the channels'."""
+    m = _module(2, 6, 16, 32, activation="silu")
+    m.weight = torch.nn.Parameter(torch.linspace(0.5, 1.5, 12, device="cuda")[::2])
+    m.bias = torch.nn.Parameter(torch.linspace(-1, 1, 18, device="cuda")[::3])
+    x, dy = _inputs((2, 6, 16, 32), torch.float32, "planes")
+    _compare(_step(m, x, dy), *_exact(m, x, dy))
+    one = torch.full((1,), 0.75, device="cuda", requires_grad=True)
+    y = torch.func.functional_call(m, {"weight": one.expand(6), "bias": m.bias}, (x,))
+    (got,) = torch.autograd.grad(y, (one,), dy)
+    with torch.no_grad():
+        m.weight.fill_(0.75)
+    want, tol = _exact(m, x, dy)
+    # (six channels' gradients, each a float32 value, and five additions of them: 6 half steps of the sum of the sizes)
+    bound = tol[2].sum() + 6 * HALF[torch.float32] * want[2].abs().sum()
+    assert (got.double() - want[2].sum()).abs() <= bound
+    m.weight = torch.nn.Parameter(torch.ones(5, device="cuda"))
+    with pytest.raises(RuntimeError, match="of shape"):
+        m(x)

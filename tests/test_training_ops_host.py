@@ -140,3 +140,28 @@ def test_oracle_agrees_on_the_quadrature():
     _, w = orc.colatitudes(13, "legendre-gauss")
     m = th.GroupNormS2(1, 1, (13, 24), grid="legendre-gauss")
     assert np.allclose(m.lat_weights.double().numpy(), w / np.mean(w), rtol=1e-6)
+
+
+def test_replaced_parameters_are_checked():
+    def module(weight, bias):
+        m = th.GroupNormS2(2, 4, (13, 24))
+        m.weight = None if weight is None else torch.nn.Parameter(weight)
+        m.bias = None if bias is None else torch.nn.Parameter(bias)
+        return m
+
+    cpu = torch.device("cpu")
+    assert module(None, None)._affine(cpu) == (None, None)
+    for weight, bias in ((torch.ones(3), torch.ones(4)), (torch.ones(4), torch.ones(5)), (torch.ones(()), torch.ones(4)), (torch.ones(1, 4), torch.ones(1, 4))):
+        with pytest.raises(RuntimeError, match="of shape"):
+            module(weight, bias)._affine(cpu)
+    for weight, bias in ((None, torch.ones(4)), (torch.ones(4), None)):
+        with pytest.raises(RuntimeError, match="both be there"):
+            module(weight, bias)._affine(cpu)
+    with pytest.raises(TypeError, match="must both be"):
+        module(torch.ones(4), torch.ones(4).half())._affine(cpu)
+    with pytest.raises(RuntimeError, match="weight on cpu"):
+        module(torch.ones(4), torch.ones(4))._affine(torch.device("cuda", 0))
+    # read as they are laid out: every other value, one value for all
+    weight, bias = module(torch.arange(8.0)[::2], torch.full((1,), 3.0).expand(4))._affine(cpu)
+    assert weight.is_contiguous() and bias.is_contiguous()
+    assert weight.tolist() == [0.0, 2.0, 4.0, 6.0] and bias.tolist() == [3.0] * 4

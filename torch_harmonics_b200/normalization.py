@@ -170,6 +170,21 @@ class GroupNormS2(nn.Module):
         state = super().__getstate__() if hasattr(super(), "__getstate__") else self.__dict__
         return {**state, "_calls": {}}
 
+    def _affine(self, device):
+        """``weight`` and ``bias`` as the kernels read them.  They may have been replaced since the module was made."""
+        weight, bias = self.weight, self.bias
+        if weight is None and bias is None:
+            return None, None
+        if weight is None or bias is None:
+            raise RuntimeError("GroupNormS2: weight and bias must both be there, or neither")
+        if weight.device != device or bias.device != device:
+            raise RuntimeError(f"GroupNormS2: the input is on {device}, weight on {weight.device}, bias on {bias.device}")
+        if weight.dtype not in _DTYPES or bias.dtype != weight.dtype:
+            raise TypeError(f"GroupNormS2: weight and bias must both be float32, bfloat16 or float16, got {weight.dtype} and {bias.dtype}")
+        if weight.shape != (self.num_channels,) or bias.shape != (self.num_channels,):
+            raise RuntimeError(f"GroupNormS2: expected weight and bias of shape ({self.num_channels},), got {tuple(weight.shape)} and {tuple(bias.shape)}")
+        return weight.contiguous(), bias.contiguous()  # (one value expanded to all channels is a copy here, and its gradient a sum)
+
     def _call(self, x, weight):
         """(descriptor, workspace bytes forward, backward) of a call on ``x``: shapes and types only."""
         param = torch.float32 if weight is None else weight.dtype
@@ -195,12 +210,7 @@ class GroupNormS2(nn.Module):
             raise RuntimeError(f"Expected tensor with 4 dimensions but got {x.dim()} instead")
         if x.shape[1:] != (self.num_channels, self.nlat, self.nlon):
             raise RuntimeError(f"Expected shape (batch, {self.num_channels}, {self.nlat}, {self.nlon}), got {tuple(x.shape)}")
-        weight, bias = self.weight, self.bias
-        if weight is not None:
-            if weight.device != x.device or bias.device != x.device:
-                raise RuntimeError(f"GroupNormS2: the input is on {x.device}, the parameters on {weight.device}")
-            if weight.dtype not in _DTYPES or bias.dtype != weight.dtype:
-                raise TypeError(f"GroupNormS2: weight and bias must both be float32, bfloat16 or float16, got {weight.dtype} and {bias.dtype}")
+        weight, bias = self._affine(x.device)
         lat = self._buffers["lat_weights"]
         if lat is not None and lat.device != x.device:
             raise RuntimeError(f"GroupNormS2: the input is on {x.device}, the latitude weights on {lat.device}")
