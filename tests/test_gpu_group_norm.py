@@ -524,3 +524,17 @@ def test_replaced_parameters():
     m.weight = torch.nn.Parameter(torch.ones(5, device="cuda"))
     with pytest.raises(RuntimeError, match="of shape"):
         m(x)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("fmt", ["planes", "last"])
+@pytest.mark.parametrize("rows", ["first", "last", "all_but_one", "every_other"])
+def test_rows_of_weight_zero(rows, fmt, dtype):
+    """Rows that do not count: what they hold, far out here, changes no statistics; they are normalised like the others."""
+    m = _module(2, 6, 20, 48, activation="gelu")
+    _parameters(m)
+    none = {"first": slice(0, 13), "last": slice(11, 20), "all_but_one": slice(0, 19), "every_other": slice(0, 20, 2)}[rows]
+    m.lat_weights[none] = 0.0
+    x, dy = _inputs((2, 6, 20, 48), dtype, fmt)
+    x[:, :, none] += 3
+    _compare(_step(m, x, dy), *_exact(m, x, dy))

@@ -608,7 +608,7 @@ template <typename T> __device__ __forceinline__ void accumulate(const F2 (&v)[k
 }
 __device__ __forceinline__ F2 reciprocal(F2 a) {
     const float2 v = split(a);
-    return f2(__fdividef(1.f, v.x), __fdividef(1.f, v.y));
+    return f2(v.x > 0.f ? __fdividef(1.f, v.x) : 0.f, v.y > 0.f ? __fdividef(1.f, v.y) : 0.f);  // (0 while all rows so far have weight 0)
 }
 // sums about c + delta from those about c
 __device__ __forceinline__ void recentre(F2 W, F2 delta, F2 &S1, F2 &S2) {
