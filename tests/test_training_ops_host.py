@@ -159,7 +159,7 @@ def test_replaced_parameters_are_checked():
             module(weight, bias)._affine(cpu)
     with pytest.raises(TypeError, match="must both be"):
         module(torch.ones(4), torch.ones(4).half())._affine(cpu)
-    with pytest.raises(RuntimeError, match="weight on cpu"):
+    with pytest.raises(RuntimeError, match="the parameters on cpu"):
         module(torch.ones(4), torch.ones(4))._affine(torch.device("cuda", 0))
     # read as they are laid out: every other value, one value for all
     weight, bias = module(torch.arange(8.0)[::2], torch.full((1,), 3.0).expand(4))._affine(cpu)

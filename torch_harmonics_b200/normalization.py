@@ -178,7 +178,7 @@ class GroupNormS2(nn.Module):
         if weight is None or bias is None:
             raise RuntimeError("GroupNormS2: weight and bias must both be there, or neither")
         if weight.device != device or bias.device != device:
-            raise RuntimeError(f"GroupNormS2: the input is on {device}, weight on {weight.device}, bias on {bias.device}")
+            raise RuntimeError(f"GroupNormS2: the input is on {device}, the parameters on {weight.device} and {bias.device}")
         if weight.dtype not in _DTYPES or bias.dtype != weight.dtype:
             raise TypeError(f"GroupNormS2: weight and bias must both be float32, bfloat16 or float16, got {weight.dtype} and {bias.dtype}")
         if weight.shape != (self.num_channels,) or bias.shape != (self.num_channels,):
