@@ -276,3 +276,21 @@ def test_refusals():
         th.global_norm([g.double()])
     with pytest.raises(TypeError, match="dense"):
         th.global_norm([g.to_sparse()])
+
+
+def test_slices_of_one_tensor():
+    """Columns of one tensor, neither of them gapless: clipped apart from one another, refused where they share a column."""
+    import torch_harmonics_b200 as th
+
+    base = _tensors([((6, 10), F32)])[0]
+    old = base.clone()
+    ps = [torch.nn.Parameter(torch.zeros(6, n, device="cuda")) for n in (4, 6)]
+    ps[0].grad, ps[1].grad = base[:, :4], base[:, 4:]
+    th.clip_grad_norm_(ps, 0.5)
+    _clipped_right([base], [old], _norm([old], 2.0), 0.5)
+    ps[1].grad = base[:, 3:9]
+    old = base.clone()
+    for clip in (lambda: th.clip_grad_norm_(ps, 0.5), lambda: th.clip_grads_with_norm_(ps, 0.5, torch.tensor(3.0, device="cuda"))):
+        with pytest.raises(RuntimeError, match="share memory"):
+            clip()
+    assert torch.equal(base, old)

@@ -165,3 +165,53 @@ def test_replaced_parameters_are_checked():
     weight, bias = module(torch.arange(8.0)[::2], torch.full((1,), 3.0).expand(4))._affine(cpu)
     assert weight.is_contiguous() and bias.is_contiguous()
     assert weight.tolist() == [0.0, 2.0, 4.0, 6.0] and bias.tolist() == [3.0] * 4
+
+
+def _bytes_of(t):
+    at = torch.zeros((), dtype=torch.int64)
+    for st, n in zip(t.stride(), t.shape):
+        at = at.unsqueeze(-1) + st * torch.arange(n)
+    at = (at * t.element_size() + t.data_ptr()).flatten().tolist()
+    return {a + i for a in at for i in range(t.element_size())}
+
+
+def test_shared_memory_is_found_exactly():
+    """Against the sets of bytes: boxes of a tensor in any place, with steps, axes in any order, and of two element sizes."""
+    from torch_harmonics_b200.gradients import _share
+
+    gen = np.random.default_rng(0)
+    base = torch.zeros(7, 9, 11)
+    half = base.view(torch.bfloat16)
+
+    def box():
+        t = base if gen.integers(3) else half
+        sl = []
+        for n in t.shape:
+            lo = int(gen.integers(n))
+            sl.append(slice(lo, int(gen.integers(lo, n)) + 1, int(gen.integers(1, 4))))
+        return t[tuple(sl)].permute(*gen.permutation(3).tolist())
+
+    seen = set()
+    for _ in range(2000):
+        a, b = box(), box()
+        want = bool(_bytes_of(a) & _bytes_of(b))
+        seen.add(want)
+        assert _share(a, b) == want and _share(b, a) == want, (a.shape, a.stride(), a.storage_offset(), b.shape, b.stride(), b.storage_offset())
+    assert seen == {True, False}
+
+
+def test_slices_that_share_memory_are_refused():
+    from torch_harmonics_b200.gradients import _refuse_shared
+
+    bucket = torch.zeros(6, 10)
+    left, right = bucket[:, :4], bucket[:, 4:]
+
+    def check(*grads):
+        _refuse_shared(list(grads), [g if g.is_contiguous() else g.contiguous() for g in grads], "clip_grad_norm_")
+
+    check(left, right, torch.zeros(3))
+    check(bucket[0], bucket[1:, 2:], torch.zeros(0))
+    check(bucket[::2, 1:], bucket[1::2, 1:])
+    for grads in ((left, left), (left, bucket[:, 3:]), (bucket, right), (bucket[1], left, right), (torch.zeros(2), bucket.t()[2:5], right)):
+        with pytest.raises(RuntimeError, match="share memory"):
+            check(*grads)

@@ -54,6 +54,51 @@ def _fills_memory(t):
     return True
 
 
+def _extent(t):
+    """First byte of ``t`` and the one behind its last."""
+    return t.data_ptr(), t.data_ptr() + (1 + sum(st * (n - 1) for st, n in zip(t.stride(), t.shape))) * t.element_size()
+
+
+def _share(a, b):
+    """Whether ``a`` and ``b`` have a byte in common: is there a solution of ``sum stride_k t_k = distance`` with every ``t_k``, a difference of
+    two indices, in its range?  (Strides of slices are nested: one or two values of each have to be tried.)"""
+    spans = {}
+    for t, lo, hi in ((a, 0, 1), (b, -1, 0)):
+        for st, n in (*zip((st * t.element_size() for st in t.stride()), t.shape), (1, t.element_size())):
+            if st and n > 1:
+                at = spans.setdefault(st, [0, 0])
+                at[0] += lo * (n - 1)
+                at[1] += hi * (n - 1)
+    spans = sorted(((st, *at) for st, at in spans.items()), reverse=True)
+    tries = 10000
+
+    def solve(k, rest):
+        nonlocal tries
+        if k == len(spans):
+            return rest == 0
+        st, lo, hi = spans[k]
+        least, most = (sum(q * span[i] for q, *span in spans[k + 1 :]) for i in (0, 1))
+        for t in range(max(lo, -((most - rest) // st)), min(hi, (rest - least) // st) + 1):
+            tries -= 1
+            if tries < 0 or solve(k + 1, rest - st * t):  # (strides that need so many are taken to share)
+                return True
+        return False
+
+    return solve(0, b.data_ptr() - a.data_ptr())
+
+
+def _refuse_shared(grads, copies, what):
+    """Tensors that are scaled as a copy are written back whole: raise where one shares memory with another tensor.  (Those that are
+    scaled where they are are compared by the library.)"""
+    held = sorted(((*_extent(g), g, g is not c) for g, c in zip(grads, copies) if g.numel()), key=lambda e: e[0])
+    near = []  # that reach beyond the first byte of the one at hand
+    for lo, hi, g, copied in held:
+        near = [e for e in near if e[0] > lo]
+        if any((copied or other) and _share(h, g) for _, h, other in near):
+            raise RuntimeError(f"{what}: two of the gradients share memory")
+        near.append((hi, g, copied))
+
+
 def _refuse(tensors, what):
     """Raise for the first tensor that cannot be taken."""
     for t in tensors:
@@ -133,7 +178,9 @@ def _grads(parameters):
     return [g for g in map(_get_grad, parameters) if g is not None]
 
 
-def _clip_in_place(grads, ls, max_norm, kind, norm=None):
+def _clip_in_place(grads, ls, max_norm, kind, what, norm=None):
+    if ls.tensors is not grads:
+        _refuse_shared(grads, ls.tensors, what)
     norm = _clip(ls, None, max_norm, kind, norm)
     if ls.tensors is not grads:
         for g, h in zip(grads, ls.tensors):
@@ -169,7 +216,7 @@ def clip_grad_norm_(
     if error_if_nonfinite:
         norm = _norm(ls, kind)
         _refuse_nonfinite(norm, norm_type)
-    return _clip_in_place(grads, ls, max_norm, kind, norm)
+    return _clip_in_place(grads, ls, max_norm, kind, "clip_grad_norm_", norm)
 
 
 @torch.no_grad()
@@ -182,7 +229,7 @@ def clip_grads_with_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]
     ls = _List(grads, "clip_grads_with_norm_")
     if total_norm.numel() != 1 or total_norm.device != grads[0].device:
         raise RuntimeError(f"clip_grads_with_norm_: expected total_norm as a scalar on {grads[0].device}, got shape {tuple(total_norm.shape)} on {total_norm.device}")
-    _clip_in_place(grads, ls, max_norm, _lib.NORM_L2, total_norm.to(torch.float32).contiguous())
+    _clip_in_place(grads, ls, max_norm, _lib.NORM_L2, "clip_grads_with_norm_", total_norm.to(torch.float32).contiguous())
 
 
 @torch.no_grad()
