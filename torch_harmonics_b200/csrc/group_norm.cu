@@ -357,6 +357,38 @@ __device__ __forceinline__ void advance(const GnArgs &a, Rows &r) {
         ++r.row;
     }
 }
+// Weights of the U vectors of a whole round, r and w moved on to the next one.  False, and nothing moved, where the vectors have to be taken one at
+// a time.
+// Planes look every vector's weight up, unless one lies across a row's end: a warp's round spans a third of a row of 1440 16-bit values, so a
+// branch for rounds within a row is taken both ways too often (721x1440x64 bf16, forward / backward: 85 / 136 us, with the branch 89 / 148).
+// Channels last a round spans a few points: those within a row share a weight, the others go one at a time (361x720x256 bf16: 87 / 134 us,
+// looked up 88 / 137).
+template <int U, bool PLANES> __device__ __forceinline__ bool round_weights(const GnArgs &a, int have, Rows &r, float &w, float (&wu)[U]) {
+    if (have < U) return false;
+    if (!a.lat || (!PLANES && r.col + U * a.step_px + r.over < a.nlon)) {  // all in one row, the next one too
+#pragma unroll
+        for (int u = 0; u < U; ++u) wu[u] = w;
+        r.col += U * a.step_px;
+        return true;
+    }
+    if constexpr (PLANES) {
+        Rows q = r;
+        float v = w;
+        bool across = false;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            wu[u] = v;
+            across |= q.col + q.over >= a.nlon;
+            advance(a, q);
+            v = __ldg(a.lat + min(q.row, a.nlat - 1));
+        }
+        if (across) return false;
+        r = q;
+        w = v;
+        return true;
+    }
+    return false;
+}
 // weights of the slots of a vector across a row's end
 template <typename T> __device__ __forceinline__ void mixed_weights(const float *lat, int nlon, int cu, int ch, int row, int col, float (&w)[kV<T>]) {
 #pragma unroll
@@ -621,7 +653,8 @@ constexpr int kUnroll = 2;
 template <typename T> constexpr int kStatsCtas = sizeof(T) == 4 ? 4 : 3;  // on an SM: 8 slots a thread spill at 4 (73 channels bf16 126 us, at 3 101); 4 slots do not
 using StatsFeed = Feed<1, kUnroll, 3>;  // (721x1440x73 bf16 channels last, forward: 101 us with 3 rounds, 103 with 2, 107 with 5)
 
-// Sums of a chunk.  Bound by reading x in float32; with 16-bit values by the instructions per value (convert, subtract, two sums in pairs).
+// Sums of a chunk.  Bound by reading x in float32.  With 16-bit values a vector has twice the arithmetic: at 24 warps an SM 59 % of the issue slots are
+// taken and most warps wait for a result of their own (without the weights' multiplications it is no faster).
 // 721x1440x73 float32 planes, with the pass below: 165 us, 5.5 TB/s over two reads and a write.
 
 template <typename T, bool PLANES> __global__ void __launch_bounds__(kThreads, kStatsCtas<T>) gn_stats_kernel(const __grid_constant__ GnArgs a) {
@@ -673,19 +706,17 @@ template <typename T, bool PLANES> __global__ void __launch_bounds__(kThreads, k
                     if (a.lat && 2 * r.row < a.nlat && have == U) unpack(raw[U - 1], c, T());
                 }
                 feed.next();
-                if (have == U && (!a.lat || r.col + U * a.step_px + r.over < a.nlon)) {  // all in one row, the next one too
-                    const F2 w2 = f2(w);
-                    F2 wp[P];
-#pragma unroll
-                    for (int p = 0; p < P; ++p) wp[p] = w2;
+                float wu[U];
+                if (round_weights<U, PLANES>(a, have, r, w, wu)) {
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
-                        F2 v[P];
+                        F2 v[P], wp[P];
                         unpack(raw[u], v, T());
+#pragma unroll
+                        for (int p = 0; p < P; ++p) wp[p] = f2(wu[u]);
                         accumulate<T>(v, c, q, wp);
+                        W += wu[u];
                     }
-                    W = fmaf((float)U, w, W);
-                    r.col += U * a.step_px;
                 } else {
 #pragma unroll
                     for (int u = 0; u < U; ++u)
@@ -978,8 +1009,8 @@ template <typename T, int ACT> __device__ __forceinline__ float2 ragged_slope(co
 }
 
 // (sum g, sum g xh) of the channels of a chunk: the slope is evaluated here and again in the second pass, since storing g would cost a write and a
-// read of the field.  721x1440x64 float32 planes, with the pass below: 230 us, 5.8 TB/s over four reads and a write; 16-bit values are bound
-// by the slope's arithmetic (73 channels bf16: 155 us, 4.9 TB/s).
+// read of the field.  721x1440x64 float32 planes, with the pass below: 230 us, 5.8 TB/s over four reads and a write; with 16-bit values
+// the registers that 8 slots take leave 16 warps an SM, which wait for their own results (73 channels bf16: 153 us, 4.9 TB/s, 49 % of the issue slots).
 template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_sums_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kUnrollB;
     __shared__ __align__(16) F2 red[PLANES ? kWarps : P * kThreads];
@@ -1300,13 +1331,14 @@ template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kT
             }
             feed.next();
             F2 wt[P];
-            if (have == U && (!a.lat || r.col + U * a.step_px + r.over < a.nlon)) {  // all in one row, the next one too
-                const F2 w2 = f2(w);
+            float wu[U];
+            if (round_weights<U, PLANES>(a, have, r, w, wu)) {
 #pragma unroll
-                for (int p = 0; p < P; ++p) wt[p] = w2;
+                for (int u = 0; u < U; ++u) {
 #pragma unroll
-                for (int u = 0; u < U; ++u) to[u * step] = one(rx[u], rd[u], wt);
-                r.col += U * a.step_px;
+                    for (int p = 0; p < P; ++p) wt[p] = f2(wu[u]);
+                    to[u * step] = one(rx[u], rd[u], wt);
+                }
             } else {
 #pragma unroll
                 for (int u = 0; u < U; ++u)
