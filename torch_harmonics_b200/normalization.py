@@ -111,6 +111,9 @@ class GroupNormS2(nn.Module):
     where they are, other strides are copied first.  The output has the input's type and layout; statistics, sums and the
     activation are float32 or wider whatever the type, under autocast too.  The parameters may have any of the three types.  The
     gradients can be computed once (no second derivatives).
+
+    Calls may be captured into a CUDA graph.  A backward pass is captured only while no autograd graph of an eager step on the same
+    parameters is alive (delete its loss first): torch accumulates gradients on the stream of that step, which ends the capture.
     """
 
     def __init__(
