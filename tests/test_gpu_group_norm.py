@@ -538,3 +538,40 @@ def test_rows_of_weight_zero(rows, fmt, dtype):
     x, dy = _inputs((2, 6, 20, 48), dtype, fmt)
     x[:, :, none] += 3
     _compare(_step(m, x, dy), *_exact(m, x, dy))
+
+
+@pytest.mark.parametrize("fmt", ["planes", "last"])
+@pytest.mark.parametrize("dtype,level", [(torch.float32, 101376.0), (torch.bfloat16, 101376.0), (torch.float16, 60000.0), (torch.float16, 1000.0)], ids=["f32", "bf16", "f16", "f16_low"])
+def test_constant_fields_give_the_shift_in_every_type(dtype, level, fmt):
+    """A constant field has the variance 0: r = eps^(-1/2) multiplies what is left of x - mean, which has to be nothing at all."""
+    m = _module(2, 6, 19, 37, affine=True)
+    _parameters(m)
+    x = torch.full((2, 6, 19, 37), level, device="cuda", dtype=dtype).contiguous(memory_format=FORMATS[fmt])
+    _, dy = _inputs((2, 6, 19, 37), dtype, fmt)
+    got = _step(m, x, dy)
+    assert torch.equal(got[0], m.bias.to(dtype).view(1, 6, 1, 1).expand_as(got[0]))
+    _compare(got, *_exact(m, x, dy))
+
+
+@pytest.mark.parametrize("fmt", ["planes", "last"])
+@pytest.mark.parametrize("act", [None, "silu", "gelu"])
+@pytest.mark.parametrize("dtype,level,step", [(torch.bfloat16, 101376.0, 512.0), (torch.float16, 60000.0, 32.0), (torch.float16, 1000.0, 0.5)], ids=["bf16", "f16", "f16_low"])
+def test_one_step_at_one_point(dtype, level, step, act, fmt):
+    """Fields that are constant but for the smallest possible step of their type at one of 20,200 points."""
+    m = _module(6, 6, 101, 200, activation=act, grid="legendre-gauss")
+    _parameters(m)
+    x = torch.full((1, 6, 101, 200), level, device="cuda", dtype=dtype)
+    x[:, :, 33, 77] += step
+    x = x.contiguous(memory_format=FORMATS[fmt])
+    _, dy = _inputs((1, 6, 101, 200), dtype, fmt)
+    _compare(_step(m, x, dy), *_exact(m, x, dy))
+
+
+@pytest.mark.parametrize("fmt", ["planes", "last"])
+@pytest.mark.parametrize("dtype,level", [(torch.bfloat16, 1.0e3), (torch.float16, 1.0e3), (torch.float16, 3.0e4)], ids=["bf16", "f16", "f16_high"])
+def test_level_far_above_spread_in_16_bits(dtype, level, fmt):
+    """As with float32 above: the inputs, here a few steps of the type apart, are what is normalised, so the bound is the same."""
+    m = _module(2, 6, 61, 120, activation="gelu")
+    _parameters(m)
+    x, dy = _inputs((2, 6, 61, 120), dtype, fmt, level=level)
+    _compare(_step(m, x, dy), *_exact(m, x, dy))
