@@ -575,3 +575,30 @@ def test_level_far_above_spread_in_16_bits(dtype, level, fmt):
     _parameters(m)
     x, dy = _inputs((2, 6, 61, 120), dtype, fmt, level=level)
     _compare(_step(m, x, dy), *_exact(m, x, dy))
+
+
+@pytest.mark.parametrize("fmt", ["planes", "last"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+def test_tail_of_gelu_relative_to_itself(dtype, fmt):
+    """gelu of z between -13 and 0, where it falls to 1e-37, against itself rather than against 1.
+
+    z carries the error t = F (1 + |xh w| + |b|) of float32 above.  The logarithmic slope of z Phi(z) is 1 / z + phi(z) / Phi(z), and for z = -a the second
+    term lies below (a + sqrt(a^2 + 4)) / 2 <= a + 1 (Mills' ratio), so it is at most |z| + 1 + 1 / |z|.  e^(-z^2 / 2) has an argument of three
+    roundings (1.5 z^2 x 2^-24) and an error of 2^-22 of its own, the rest of the product is ten roundings or so: 2^-21 (1 + z^2) together.  The fit is off by
+    1.3e-7 (2^-22) before float32 and by 2.9e-5 (2^-15) before 16 bits."""
+    m = _module(4, 8, 91, 180, activation="gelu")
+    with torch.no_grad():
+        m.weight.fill_(2.0)
+        m.bias.copy_(torch.linspace(-6, -1, 8))
+    x, dy = _inputs((2, 8, 91, 180), dtype, fmt)
+    (e, *_), (t, *_) = _exact(m, x, dy)
+    m.activation = None
+    z = _exact(m, x, dy)[0][0]
+    m.activation = "gelu"
+    got = m(x).double()
+    fit = {torch.float32: 2.0**-22, torch.bfloat16: 2.0**-15, torch.float16: 2.0**-15}[dtype]
+    bound = (HALF[dtype] + t * (z.abs() + 1 + 1 / z.abs()) + 2.0**-21 * (1 + z * z) + fit) * e.abs() + TINY[dtype]
+    low = (z < -1e-3) & (z > -13.0)
+    assert low.sum() > 100_000
+    d = ((got - e).abs() / bound)[low]
+    assert (d <= 1).all(), f"{float(d.max()):.2f} times the bound"

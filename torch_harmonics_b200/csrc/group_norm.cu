@@ -86,23 +86,32 @@ __device__ __forceinline__ float rcp_fast(float x) {
 // ------------------------------------------------------------------------------------------------
 // Normal distribution function of -|z|:  Phi(-a) = e^(-a^2 / 2) R(a),  R(a) = t P(t) with t = 1 / (1 + 0.3 a): the polynomial P of
 // degree 7 is the minimax fit of R(a) / t in relative error over 0 <= a <= 13.5 (1.3e-7; computed by reweighted least squares
-// against the scaled complementary error function).  Values that are rounded to 16 bits behind it take degree 5 and 1 / (1 + 0.31 a) (4.6e-6, a
-// hundredth of float16's half step).  gelu(z) = max(z, 0) - a Phi(-a) then keeps its relative accuracy in both tails.
+// against the scaled complementary error function).  gelu(z) = max(z, 0) - a Phi(-a) then keeps its relative accuracy in the tail, up to the rounding of
+// z^2: 2e-6 at z = -6.  Values that are rounded to 16 bits behind it take degree 4 and t = 1 / (1 + 0.375 a), 2.9e-5: an eighth of float16's smallest
+// half step.
 struct Tail {
     F2 e, r, na;  // e^(-a^2 / 2), R(a), -a
 };
-__device__ __forceinline__ Tail normal_tail(F2 z) {
+template <typename T> __device__ __forceinline__ Tail normal_tail(F2 z) {
     Tail k;
     k.na.v = z.v | 0x8000000080000000ull;
-    const float2 d = split(fma2(k.na, f2(-0.3f), f2(1.f)));
+    const float2 d = split(fma2(k.na, f2(sizeof(T) == 2 ? -0.375f : -0.3f), f2(1.f)));
     const F2 t = f2(rcp_fast(d.x), rcp_fast(d.y));
-    F2 p = fma2(t, f2(0.035931703f), f2(-0.15827584f));
-    p = fma2(t, p, f2(0.20820633f));
-    p = fma2(t, p, f2(-0.05539357f));
-    p = fma2(t, p, f2(0.12946904f));
-    p = fma2(t, p, f2(0.099637546f));
-    p = fma2(t, p, f2(0.12079835f));
-    p = fma2(t, p, f2(0.11962639f));
+    F2 p;
+    if constexpr (sizeof(T) == 2) {
+        p = fma2(t, f2(-0.090985179f), f2(0.20104314f));
+        p = fma2(t, p, f2(0.082974225f));
+        p = fma2(t, p, f2(0.15792f));
+        p = fma2(t, p, f2(0.14904104f));
+    } else {
+        p = fma2(t, f2(0.035931703f), f2(-0.15827584f));
+        p = fma2(t, p, f2(0.20820633f));
+        p = fma2(t, p, f2(-0.05539357f));
+        p = fma2(t, p, f2(0.12946904f));
+        p = fma2(t, p, f2(0.099637546f));
+        p = fma2(t, p, f2(0.12079835f));
+        p = fma2(t, p, f2(0.11962639f));
+    }
     k.r = mul2(t, p);
     const float2 x = split(mul2(mul2(z, f2(-0.72134752f)), z));
     k.e = f2(exp2_fast(x.x), exp2_fast(x.y));
@@ -114,9 +123,6 @@ __device__ __forceinline__ F2 logistic(F2 z) {
     return f2(rcp_fast(d.x), rcp_fast(d.y));
 }
 
-// (gelu behind 16-bit rounding takes kValueScale z:  y = z / 2 - a (1/2 - e^(-a^2 / 2) R(a)), two operations less; what this loses of the
-// far tail, 1e-7 |z|, is far below the rounding)
-template <typename T, int ACT> constexpr float kValueScale = ACT == SHTB200_ACT_GELU && sizeof(T) == 2 ? 0.84932180f : 1.f;
 template <typename T, int ACT> __device__ __forceinline__ F2 act_value(F2 z) {
     if constexpr (ACT == SHTB200_ACT_RELU) {
         const float2 v = split(z);
@@ -124,24 +130,9 @@ template <typename T, int ACT> __device__ __forceinline__ F2 act_value(F2 z) {
     } else if constexpr (ACT == SHTB200_ACT_SILU) {
         return mul2(z, logistic(z));
     } else if constexpr (ACT == SHTB200_ACT_GELU) {
-        if constexpr (sizeof(T) == 2) {
-            constexpr float F = 1.f / kValueScale<T, ACT>;
-            F2 na;
-            na.v = z.v | 0x8000000080000000ull;
-            const float2 d = split(fma2(na, f2(-0.31f * F), f2(1.f)));
-            const F2 t = f2(rcp_fast(d.x), rcp_fast(d.y));
-            F2 r = fma2(t, f2(-0.07392906f * F), f2(0.1804501f * F));
-            r = fma2(t, r, f2(0.015744982f * F));
-            r = fma2(t, r, f2(0.13342965f * F));
-            r = fma2(t, r, f2(0.12044131f * F));
-            r = fma2(t, r, f2(0.1238607f * F));
-            const float2 x = split(mul2(z, z));
-            return fma2(na, fma2(f2(exp2_fast(-x.x), exp2_fast(-x.y)), mul2(t, r), f2(-0.5f * F)), mul2(z, f2(0.5f * F)));
-        } else {
-            const Tail k = normal_tail(z);
-            const float2 v = split(z);
-            return fma2(k.na, mul2(k.e, k.r), f2(fmaxf(v.x, 0.f), fmaxf(v.y, 0.f)));
-        }
+        const Tail k = normal_tail<T>(z);
+        const float2 v = split(z);
+        return fma2(mul2(k.na, k.e), k.r, f2(fmaxf(v.x, 0.f), fmaxf(v.y, 0.f)));
     }
     return z;
 }
@@ -941,9 +932,8 @@ template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kT
 #pragma unroll
             for (int p = 0; p < P; ++p) {
                 const float4 u = st[g[2 * p]], v = st[g[2 * p + 1]];
-                constexpr float F = kValueScale<T, ACT>;
-                sc[p] = mul2(f2(u.z * F, v.z * F), f2(w[2 * p], w[2 * p + 1]));
-                sh[p] = fma2(f2(-u.y, -v.y), sc[p], f2(b[2 * p] * F, b[2 * p + 1] * F));
+                sc[p] = mul2(f2(u.z, v.z), f2(w[2 * p], w[2 * p + 1]));
+                sh[p] = fma2(f2(-u.y, -v.y), sc[p], f2(b[2 * p], b[2 * p + 1]));
                 m[p] = f2(u.x, v.x);
             }
         }
@@ -979,7 +969,7 @@ template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kT
             const int ch = e % a.cu, c = a.cl ? ch : k.c;
             const float4 v = st[ch / a.cgu];
             const float sc = v.z * load_param(a.weight, a.pdtype, c, 1.f), sh = fmaf(-v.y, sc, load_param(a.bias, a.pdtype, c, 0.f));
-            store_f(y + e, split(act_value<T, ACT>(f2(kValueScale<T, ACT> * fmaf(to_f(x[e]) - v.x, sc, sh)))).x);
+            store_f(y + e, split(act_value<T, ACT>(f2(fmaf(to_f(x[e]) - v.x, sc, sh)))).x);
         }
     }
 }
