@@ -602,3 +602,13 @@ def test_tail_of_gelu_relative_to_itself(dtype, fmt):
     assert low.sum() > 100_000
     d = ((got - e).abs() / bound)[low]
     assert (d <= 1).all(), f"{float(d.max()):.2f} times the bound"
+
+
+@pytest.mark.parametrize("fmt", ["planes", "last"])
+@pytest.mark.parametrize("far,rows,channels", [(1.0e4, 1, 73), (1.0e3, 2, 73), (1.0e4, 1, 3), (1.0e5, 1, 32)])
+def test_first_rows_far_out(far, rows, channels, fmt):
+    """The rows at the pole, a millionth of the weight, are far out (a missing value's mark) and are the first part of the sums, whose mean the others are joined about."""
+    m = _module(1, channels, 721, 1440)
+    x, dy = _inputs((1, channels, 721, 1440), torch.float32, fmt)
+    x[:, :, :rows] += far
+    _compare(_step(m, x, dy), *_exact(m, x, dy))
