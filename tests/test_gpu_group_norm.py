@@ -612,3 +612,35 @@ def test_first_rows_far_out(far, rows, channels, fmt):
     x, dy = _inputs((1, channels, 721, 1440), torch.float32, fmt)
     x[:, :, :rows] += far
     _compare(_step(m, x, dy), *_exact(m, x, dy))
+
+
+FAR = {"level": (1.0e5, 0.0), "fill": (0.0, 1.0e4), "level_and_fill": (1.0e4, -3.0e4)}
+
+
+@pytest.mark.parametrize("fmt", ["planes", "last"])
+@pytest.mark.parametrize("rows", ["first", "last", "middle", "every_other"])
+@pytest.mark.parametrize("far", list(FAR))
+def test_rows_of_weight_zero_in_fields_of_many_chunks(far, rows, fmt):
+    """Rows that do not count are whole parts of the sums here (a field is summed in hundreds of parts), the first of them too, and what they hold is far from
+    the rest, whose level may be far above its spread.  The bound is that of float32 above: relative to |xh|, so that of the counted rows is tight."""
+    level, fill = FAR[far]
+    m = _module(8, 32, 256, 512, activation="silu")
+    _parameters(m)
+    none = {"first": slice(0, 30), "last": slice(226, 256), "middle": slice(100, 150), "every_other": slice(0, 256, 2)}[rows]
+    m.lat_weights[none] = 0.0
+    x, dy = _inputs((1, 32, 256, 512), torch.float32, fmt, level=level)
+    x[:, :, none] += fill
+    _compare(_step(m, x, dy), *_exact(m, x, dy))
+
+
+@pytest.mark.parametrize("fmt", ["planes", "last"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows", [slice(0, 1), slice(0, 13), slice(11, 20), slice(0, 19), slice(0, 20, 2), slice(1, 20)], ids=str)
+def test_far_values_in_rows_of_weight_zero(rows, dtype, fmt):
+    """The same inside one part of the sums: vectors of a thread that do not count come before those that do, and lie across the ends of rows."""
+    m = _module(2, 6, 20, 45)
+    _parameters(m)
+    m.lat_weights[rows] = 0.0
+    x, dy = _inputs((2, 6, 20, 45), dtype, fmt)
+    x[:, :, rows] += 1.0e4
+    _compare(_step(m, x, dy), *_exact(m, x, dy))

@@ -25,6 +25,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <climits>
 #include <map>
 #include <mutex>
 #include <numeric>
@@ -490,8 +491,8 @@ __device__ __forceinline__ double warp_sum(double v) {
 }
 __device__ __forceinline__ double2 warp_sum(double2 v) { return make_double2(warp_sum(v.x), warp_sum(v.y)); }
 
-// Partial results joined in float64, about the mean of the first (fields whose level is far above their spread lose nothing, and no division is
-// needed on the way): thread `i` of `of` takes every of-th, four loads at a time.
+// Partial results joined in float64, about the mean of the first that has any weight (fields whose level is far above their spread lose nothing, and no
+// division is needed on the way; a part of rows that do not count has no mean): thread `i` of `of` takes every of-th, four loads at a time.
 struct Sums64 {
     double c, W, s, q;
     __device__ __forceinline__ void add(const float4 &v) {
@@ -503,15 +504,24 @@ struct Sums64 {
         }
     }
     __device__ __forceinline__ void gather(const float4 *p, int n, long long stride, int i, int of) {
-        const float4 v0 = __ldcg(p);
-        c = (double)v0.y + v0.z;
-        W = s = q = 0.;
-        for (; i < n; i += 4 * of) {
-            float4 v[4];
+        float4 v[4], v0 = __ldcg(p);
+        auto fetch = [&] {
 #pragma unroll
             for (int u = 0; u < 4; ++u) v[u] = i + u * of < n ? __ldcg(p + (i + u * of) * stride) : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+        fetch();
+        for (int from = 0; v0.x == 0.f && from < n; from += 32) {  // (the same part for every warp and CTA)
+            const int at = from + (int)(threadIdx.x & 31);
+            const float here = at < n ? __ldcg(p + at * stride).x : 0.f;
+            if (const unsigned some = __ballot_sync(0xffffffffu, here != 0.f)) v0 = __ldcg(p + (from + __ffs(some) - 1) * stride);
+        }
+        c = (double)v0.y + v0.z;
+        W = s = q = 0.;
+        while (i < n) {
 #pragma unroll
             for (int u = 0; u < 4; ++u) add(v[u]);
+            i += 4 * of;
+            fetch();
         }
         W = warp_sum(W);
         s = warp_sum(s);
@@ -641,6 +651,24 @@ __device__ __forceinline__ void recentre(F2 W, F2 delta, F2 &S1, F2 &S2) {
     S1 = sub2(S1, t);
 }
 
+// Slots that a vector (of weights w) outweighs so far take their value in it as the centre.  True while some have met no row that counts.
+template <typename T>
+__device__ __forceinline__ bool centre_on(uint4 raw, const F2 (&w)[kP<T>], float W, const F2 (*extra)[kThreads], F2 (&c)[kP<T>], F2 (&q)[2 * kP<T>]) {
+    F2 v[kP<T>];
+    unpack(raw, v, T());
+    bool open = false;
+#pragma unroll
+    for (int p = 0; p < kP<T>; ++p) {
+        const F2 Wp = add2(extra[p][threadIdx.x], f2(W));
+        const float2 so_far = split(Wp), now = split(w[p]), x = split(v[p]), d = split(sub2(v[p], c[p])), old = split(c[p]);
+        const bool b0 = now.x > so_far.x, b1 = now.y > so_far.y;
+        recentre(Wp, f2(b0 ? d.x : 0.f, b1 ? d.y : 0.f), q[p], q[kP<T> + p]);
+        c[p] = f2(b0 ? x.x : old.x, b1 ? x.y : old.y);
+        open |= (so_far.x == 0.f && now.x == 0.f) || (so_far.y == 0.f && now.y == 0.f);
+    }
+    return open;
+}
+
 constexpr int kUnroll = 2;
 template <typename T> constexpr int kStatsCtas = sizeof(T) == 4 ? 4 : 3;  // on an SM: 8 slots a thread spill at 4 (73 channels bf16 126 us, at 3 101); 4 slots do not
 using StatsFeed = Feed<1, kUnroll, 3>;  // (721x1440x73 bf16 channels last, forward: 101 us with 3 rounds, 103 with 2, 107 with 5)
@@ -679,6 +707,7 @@ template <typename T, bool PLANES> __global__ void __launch_bounds__(kThreads, k
         StatsFeed feed;
         feed.start(gn_smem, xv + s.first, nullptr, s.count, s.step);
         if (s.count) {
+            bool open = true;  // some slots have met no row that counts
             Rows r{0, 0, 0};
             float w = 1.f;
             if (a.lat) {
@@ -691,15 +720,19 @@ template <typename T, bool PLANES> __global__ void __launch_bounds__(kThreads, k
                 feed.wait();
 #pragma unroll
                 for (int u = 0; u < U; ++u) raw[u] = feed.get(u, 0);
-                // The first centre: of the first round, the vector that counts most (a value at the pole, far out, is then no centre for
-                // rows of a hundred times its weight).
-                if (j == 0) {
-                    unpack(raw[0], c, T());
-                    if (a.lat && 2 * r.row < a.nlat && have == U) unpack(raw[U - 1], c, T());
-                }
                 feed.next();
                 float wu[U];
+                // The first centre: of the first round that counts, the vector that counts most (a value at the pole, far out, is none for rows of a
+                // hundred times its weight, and one in a row that does not count is none at all).
                 if (round_weights<U, PLANES>(a, have, r, w, wu)) {
+                    if (open) {
+                        const bool last = wu[U - 1] >= wu[0];
+                        const float most = last ? wu[U - 1] : wu[0];
+                        F2 wp[P];
+#pragma unroll
+                        for (int p = 0; p < P; ++p) wp[p] = f2(most);
+                        open = centre_on<T>(last ? raw[U - 1] : raw[0], wp, W, extra, c, q);
+                    }
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
                         F2 v[P], wp[P];
@@ -714,18 +747,20 @@ template <typename T, bool PLANES> __global__ void __launch_bounds__(kThreads, k
                     for (int u = 0; u < U; ++u)
                         if (u < have) {
                             F2 v[P], wp[P];
-                            unpack(raw[u], v, T());
 #pragma unroll
                             for (int p = 0; p < P; ++p) wp[p] = f2(w);
-                            if (a.lat && r.col + r.over >= a.nlon) {
+                            const bool mixed = a.lat && r.col + r.over >= a.nlon;
+                            if (mixed) {
                                 float ws[V];
                                 mixed_weights<T>(a.lat, a.nlon, a.cu, s.ch0, r.row, r.col, ws);
 #pragma unroll
-                                for (int p = 0; p < P; ++p) {
-                                    wp[p] = f2(ws[2 * p], ws[2 * p + 1]);
-                                    extra[p][threadIdx.x] = add2(extra[p][threadIdx.x], sub2(wp[p], f2(w)));
-                                }
+                                for (int p = 0; p < P; ++p) wp[p] = f2(ws[2 * p], ws[2 * p + 1]);
                             }
+                            if (open || mixed || w > W) open = centre_on<T>(raw[u], wp, W, extra, c, q);
+                            if (mixed)
+#pragma unroll
+                                for (int p = 0; p < P; ++p) extra[p][threadIdx.x] = add2(extra[p][threadIdx.x], sub2(wp[p], f2(w)));
+                            unpack(raw[u], v, T());
                             accumulate<T>(v, c, q, wp);
                             W += w;
                             if (a.lat) {
@@ -747,16 +782,35 @@ template <typename T, bool PLANES> __global__ void __launch_bounds__(kThreads, k
         }
         // all threads of a column: about the centre of its first thread, then added (planes: of the first slot of all)
         F2 z[3 * P];  // W, S1, S2
+        bool lost = false;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const float2 v = split(c[p]);
+            z[p] = add2(extra[p][threadIdx.x], f2(W));
+            const float2 v = split(c[p]), counted = split(z[p]);
             if (s.rep == 0) {
                 centre[(2 * p) * kPitch + s.col] = v.x;
                 centre[(2 * p + 1) * kPitch + s.col] = v.y;
+                if (!PLANES || p == 0) lost |= counted.x == 0.f || (!PLANES && counted.y == 0.f);
             }
-            z[p] = add2(extra[p][threadIdx.x], f2(W));
         }
-        __syncthreads();
+        // (where that one has met only rows that do not count: of the first that has met another)
+        if (__syncthreads_or(lost && s.count)) {
+            int *first = reinterpret_cast<int *>(tot);
+            for (int i = threadIdx.x; i < (PLANES ? 1 : V * kMaxCols); i += kThreads) first[i] = INT_MAX;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float2 counted = split(z[i / 2]);
+                if (s.count && (i & 1 ? counted.y : counted.x) > 0.f) atomicMin(first + (PLANES ? 0 : i * kMaxCols + s.col), PLANES ? s.rep * V + i : s.rep);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float2 v = split(c[i / 2]);
+                if (s.count && first[PLANES ? 0 : i * kMaxCols + s.col] == (PLANES ? s.rep * V + i : s.rep)) centre[(PLANES ? 0 : i) * kPitch + s.col] = i & 1 ? v.y : v.x;
+            }
+            __syncthreads();
+        }
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             const F2 c0 = PLANES ? f2(centre[0]) : f2(centre[(2 * p) * kPitch + s.col], centre[(2 * p + 1) * kPitch + s.col]);
