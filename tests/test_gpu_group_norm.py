@@ -644,3 +644,21 @@ def test_far_values_in_rows_of_weight_zero(rows, dtype, fmt):
     x, dy = _inputs((2, 6, 20, 45), dtype, fmt)
     x[:, :, rows] += 1.0e4
     _compare(_step(m, x, dy), *_exact(m, x, dy))
+
+
+def test_replaced_latitude_weights():
+    """Weights with strides are read as they are laid out, others are refused, and a change between forward and backward is noticed."""
+    m = _module(2, 6, 16, 32)
+    x, dy = _inputs((2, 6, 16, 32), torch.float32, "planes")
+    m.lat_weights = torch.linspace(0.5, 2.0, 32, device="cuda")[::2]
+    _compare(_step(m, x, dy), *_exact(m, x, dy))
+    m.lat_weights = torch.full((1,), 3.0, device="cuda").expand(16)
+    _compare(_step(m, x, dy), *_exact(m, x, dy))
+    m.lat_weights = torch.ones(15, device="cuda")
+    with pytest.raises(RuntimeError, match="of shape"):
+        m(x)
+    m.lat_weights = torch.ones(16, device="cuda")
+    y = m(x)
+    m.lat_weights[0] = 2.0
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()

@@ -215,3 +215,29 @@ def test_slices_that_share_memory_are_refused():
     for grads in ((left, left), (left, bucket[:, 3:]), (bucket, right), (bucket[1], left, right), (torch.zeros(2), bucket.t()[2:5], right)):
         with pytest.raises(RuntimeError, match="share memory"):
             check(*grads)
+
+
+def test_replaced_latitude_weights_are_checked():
+    """The kernels read nlat float32 values one after the other: anything else would be read beyond its end or as something else."""
+    cpu = torch.device("cpu")
+
+    def lat(t):
+        m = th.GroupNormS2(2, 4, (13, 24))
+        m.lat_weights = t
+        return m._lat(cpu)
+
+    assert lat(None) is None and th.GroupNormS2(2, 4, (13, 24), weighted=False)._lat(cpu) is None
+    for bad in (torch.ones(12), torch.ones(14), torch.ones(13, 1), torch.ones(()), torch.ones(0)):
+        with pytest.raises(RuntimeError, match="of shape"):
+            lat(bad)
+    for bad in (torch.ones(13).double(), torch.ones(13).half(), torch.ones(13, dtype=torch.int32), torch.ones(13, dtype=torch.complex64)):
+        with pytest.raises(TypeError, match="float32"):
+            lat(bad)
+    with pytest.raises(RuntimeError, match="latitude weights on cpu"):
+        th.GroupNormS2(2, 4, (13, 24))._lat(torch.device("cuda", 0))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        lat(torch.ones(13, requires_grad=True))
+    # read as they are laid out: every other value, one value for all, a lazy minus sign
+    for t in (torch.arange(26.0)[::2], torch.full((1,), 3.0).expand(13), torch.view_as_complex(torch.randn(13, 2)).conj().imag):
+        got = lat(t)
+        assert got.is_contiguous() and not got.is_neg() and got.tolist() == t.tolist()

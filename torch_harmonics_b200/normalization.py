@@ -33,7 +33,7 @@ def _aligned(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _run(module, x, weight, bias, keep):
+def _run(module, x, weight, bias, lat, keep):
     """y and (with ``keep``) what the backward pass needs, for a dense ``x``."""
     desc, ws_bytes, _ = module._call(x, weight)
     batch, dev = x.shape[0], x.device
@@ -46,7 +46,7 @@ def _run(module, x, weight, bias, keep):
     at = stats.data_ptr()
     with _lib.on_device(dev.index) as stream:
         rc = _lib.load().shtb200_group_norm_forward(
-            desc, x.data_ptr(), _ptr(module._buffers["lat_weights"]), _ptr(weight), _ptr(bias), y.data_ptr(), at, ws.data_ptr() if keep else at + stats_bytes, ws_bytes, stream
+            desc, x.data_ptr(), _ptr(lat), _ptr(weight), _ptr(bias), y.data_ptr(), at, ws.data_ptr() if keep else at + stats_bytes, ws_bytes, stream
         )
     if rc != 0:
         _lib.check(rc, "shtb200_group_norm_forward")
@@ -55,10 +55,10 @@ def _run(module, x, weight, bias, keep):
 
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, module):
-        y, stats = _run(module, x, weight, bias, True)
-        ctx.save_for_backward(x, weight, bias, stats)
-        ctx.call, ctx.lat = module._call(x, weight), module._buffers["lat_weights"]
+    def forward(ctx, x, weight, bias, lat, module):
+        y, stats = _run(module, x, weight, bias, lat, True)
+        ctx.save_for_backward(x, weight, bias, lat, stats)
+        ctx.call = module._call(x, weight)
         return y
 
     @staticmethod
@@ -68,7 +68,7 @@ class _GroupNorm(torch.autograd.Function):
 
 
 def _gradients(ctx, dy):
-    x, weight, bias, stats = ctx.saved_tensors
+    x, weight, bias, lat, stats = ctx.saved_tensors
     desc, _, ws_bytes = ctx.call
     new = torch.empty_like if x.shape[0] else torch.zeros_like
     need = ctx.needs_input_grad
@@ -76,17 +76,17 @@ def _gradients(ctx, dy):
     dw = new(weight) if need[1] else None
     db = new(bias) if need[2] else None
     if x.shape[0] == 0:
-        return dx, dw, db, None
+        return dx, dw, db, None, None
     # the gradient comes in any layout (an expanded scalar, for a sum): the kernel reads it in the layout of x
     dy = _aligned(_lib.dense(dy) if not desc.channels_last else dy.resolve_neg().contiguous(memory_format=torch.channels_last))
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
     with _lib.on_device(x.device.index) as stream:
         rc = _lib.load().shtb200_group_norm_backward(
-            desc, dy.data_ptr(), x.data_ptr(), _ptr(ctx.lat), _ptr(weight), _ptr(bias), stats.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(), ws_bytes, stream
+            desc, dy.data_ptr(), x.data_ptr(), _ptr(lat), _ptr(weight), _ptr(bias), stats.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(), ws_bytes, stream
         )
     if rc != 0:
         _lib.check(rc, "shtb200_group_norm_backward")
-    return dx, dw, db, None
+    return dx, dw, db, None, None
 
 
 _guarded_gradients = once_differentiable(_gradients)
@@ -188,6 +188,21 @@ class GroupNormS2(nn.Module):
             raise RuntimeError(f"GroupNormS2: expected weight and bias of shape ({self.num_channels},), got {tuple(weight.shape)} and {tuple(bias.shape)}")
         return weight.contiguous(), bias.contiguous()  # (one value expanded to all channels is a copy here, and its gradient a sum)
 
+    def _lat(self, device):
+        """``lat_weights`` as the kernels read them.  They may have been replaced too (by a mask of rows, for instance)."""
+        lat = self.lat_weights
+        if lat is None:
+            return None
+        if lat.device != device:
+            raise RuntimeError(f"GroupNormS2: the input is on {device}, the latitude weights on {lat.device}")
+        if lat.dtype != torch.float32:
+            raise TypeError(f"GroupNormS2: lat_weights must be float32, got {lat.dtype}")
+        if lat.shape != (self.nlat,):
+            raise RuntimeError(f"GroupNormS2: expected lat_weights of shape ({self.nlat},), got {tuple(lat.shape)}")
+        if lat.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("GroupNormS2: lat_weights get no gradient, they must not require one")
+        return _lib.dense(lat)
+
     def _call(self, x, weight):
         """(descriptor, workspace bytes forward, backward) of a call on ``x``: shapes and types only."""
         param = torch.float32 if weight is None else weight.dtype
@@ -214,12 +229,10 @@ class GroupNormS2(nn.Module):
         if x.shape[1:] != (self.num_channels, self.nlat, self.nlon):
             raise RuntimeError(f"Expected shape (batch, {self.num_channels}, {self.nlat}, {self.nlon}), got {tuple(x.shape)}")
         weight, bias = self._affine(x.device)
-        lat = self._buffers["lat_weights"]
-        if lat is not None and lat.device != x.device:
-            raise RuntimeError(f"GroupNormS2: the input is on {x.device}, the latitude weights on {lat.device}")
+        lat = self._lat(x.device)
         if not (x.is_contiguous() or x.is_contiguous(memory_format=torch.channels_last)) or x.is_neg():
             x = _lib.dense(x)
         x = _aligned(x)
         if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and (weight.requires_grad or bias.requires_grad))):
-            return _GroupNorm.apply(x, weight, bias, self)
-        return _run(self, x, weight, bias, False)[0]
+            return _GroupNorm.apply(x, weight, bias, lat, self)
+        return _run(self, x, weight, bias, lat, False)[0]
