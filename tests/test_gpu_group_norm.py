@@ -662,3 +662,17 @@ def test_replaced_latitude_weights():
     m.lat_weights[0] = 2.0
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("fmt", ["planes", "last"])
+def test_parameters_with_a_lazy_minus_sign(fmt):
+    """A single channel: a view that is contiguous whatever its stride."""
+    m = _module(1, 1, 16, 32)
+    w, b = (torch.view_as_complex(torch.tensor([[0.5, v]], device="cuda")).conj().imag for v in (1.5, -0.25))
+    assert w.is_neg() and w.is_contiguous()
+    x, dy = _inputs((2, 1, 16, 32), torch.float32, fmt)
+    with torch.no_grad():
+        got = torch.func.functional_call(m, {"weight": w, "bias": b}, (x,))
+        m.weight.fill_(-1.5)
+        m.bias.fill_(0.25)
+        assert torch.equal(got, m(x))

@@ -186,7 +186,7 @@ class GroupNormS2(nn.Module):
             raise TypeError(f"GroupNormS2: weight and bias must both be float32, bfloat16 or float16, got {weight.dtype} and {bias.dtype}")
         if weight.shape != (self.num_channels,) or bias.shape != (self.num_channels,):
             raise RuntimeError(f"GroupNormS2: expected weight and bias of shape ({self.num_channels},), got {tuple(weight.shape)} and {tuple(bias.shape)}")
-        return weight.contiguous(), bias.contiguous()  # (one value expanded to all channels is a copy here, and its gradient a sum)
+        return _lib.dense(weight), _lib.dense(bias)  # (one value expanded to all channels is a copy here, and its gradient a sum)
 
     def _lat(self, device):
         """``lat_weights`` as the kernels read them.  They may have been replaced too (by a mask of rows, for instance)."""
