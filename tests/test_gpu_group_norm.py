@@ -676,3 +676,13 @@ def test_parameters_with_a_lazy_minus_sign(fmt):
         m.weight.fill_(-1.5)
         m.bias.fill_(0.25)
         assert torch.equal(got, m(x))
+
+
+def test_lazy_minus_sign_keeps_the_layout():
+    m = _module(2, 6, 16, 32)
+    x = torch.randn(2, 6, 16, 32, device="cuda").contiguous(memory_format=torch.channels_last)
+    n = torch._neg_view(x)
+    assert n.is_neg() and n.is_contiguous(memory_format=torch.channels_last)
+    with torch.no_grad():
+        y = m(n)
+    assert y.is_contiguous(memory_format=torch.channels_last) and torch.equal(y, m(-x))

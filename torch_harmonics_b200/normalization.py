@@ -230,8 +230,10 @@ class GroupNormS2(nn.Module):
             raise RuntimeError(f"Expected shape (batch, {self.num_channels}, {self.nlat}, {self.nlon}), got {tuple(x.shape)}")
         weight, bias = self._affine(x.device)
         lat = self._lat(x.device)
-        if not (x.is_contiguous() or x.is_contiguous(memory_format=torch.channels_last)) or x.is_neg():
-            x = _lib.dense(x)
+        if x.is_neg():
+            x = x.resolve_neg()
+        if not (x.is_contiguous() or x.is_contiguous(memory_format=torch.channels_last)):
+            x = x.contiguous()
         x = _aligned(x)
         if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and (weight.requires_grad or bias.requires_grad))):
             return _GroupNorm.apply(x, weight, bias, lat, self)
