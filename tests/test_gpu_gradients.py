@@ -294,3 +294,22 @@ def test_slices_of_one_tensor():
         with pytest.raises(RuntimeError, match="share memory"):
             clip()
     assert torch.equal(base, old)
+
+
+def test_expanded_gradients():
+    """One value expanded to all entries: counted as often as it is seen, clipped into a new tensor, and refused in place before any gradient is touched."""
+    import torch_harmonics_b200 as th
+
+    (a,), one = _tensors([((50,), F32)]), torch.full((1,), 2.0, device="cuda")
+    wide = one.expand(30)
+    want = _norm([a, wide], 2.0)
+    new, n = th.clip_by_global_norm([a, wide], want / 2)
+    assert abs(float(n) - want) <= 2.0**-22 * want
+    _clipped_right(new, [a, wide], want, want / 2)
+    ps = [torch.nn.Parameter(torch.zeros(k, device="cuda")) for k in (50, 30)]
+    ps[0].grad, ps[1].grad = a, wide
+    old = a.clone()
+    for clip in (lambda: th.clip_grad_norm_(ps, want / 2), lambda: th.clip_grads_with_norm_(ps, want / 2, n), lambda: th.clip_grad_norm_(ps, want / 2, error_if_nonfinite=True)):
+        with pytest.raises(RuntimeError, match="share memory"):
+            clip()
+        assert torch.equal(a, old) and float(one) == 2.0

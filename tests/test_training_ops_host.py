@@ -241,3 +241,26 @@ def test_replaced_latitude_weights_are_checked():
     for t in (torch.arange(26.0)[::2], torch.full((1,), 3.0).expand(13), torch.view_as_complex(torch.randn(13, 2)).conj().imag):
         got = lat(t)
         assert got.is_contiguous() and not got.is_neg() and got.tolist() == t.tolist()
+
+
+def test_gradients_that_overlap_themselves_are_found_exactly():
+    """Against the sets of places: strided views of up to three axes, any strides."""
+    from torch_harmonics_b200.gradients import _overlaps_itself, _refuse_shared
+
+    gen = np.random.default_rng(1)
+    base, seen = torch.zeros(2000), set()
+    for _ in range(3000):
+        n = int(gen.integers(1, 4))
+        shape, stride = (tuple(int(v) for v in gen.integers(lo, hi, n)) for lo, hi in ((1, 6), (0, 40)))
+        t = base.as_strided(shape, stride)
+        at = torch.zeros((), dtype=torch.int64)
+        for st, k in zip(stride, shape):
+            at = at.unsqueeze(-1) + st * torch.arange(k)
+        want = at.unique().numel() < t.numel()
+        seen.add(want)
+        assert _overlaps_itself(t) == want, (shape, stride)
+    assert seen == {True, False}
+    assert not _overlaps_itself(torch.zeros(0, 3).t()) and not _overlaps_itself(torch.zeros(())) and not _overlaps_itself(base[::2])
+    for bad in (torch.zeros(1).expand(5), torch.zeros(3, 1).expand(3, 4), base.as_strided((3, 3), (1, 1)), base.as_strided((4, 4), (2, 1))):
+        with pytest.raises(RuntimeError, match="share memory"):
+            _refuse_shared([torch.zeros(3), bad], [torch.zeros(3), bad.contiguous()], "clip_grad_norm_")

@@ -59,9 +59,29 @@ def _extent(t):
     return t.data_ptr(), t.data_ptr() + (1 + sum(st * (n - 1) for st, n in zip(t.stride(), t.shape))) * t.element_size()
 
 
+def _meet(spans, distance, other_than_zero=False):
+    """Whether ``sum stride_k t_k = distance`` has a solution with every ``t_k``, a difference of two indices, in its range ``lo .. hi``, for ``spans`` of
+    ``(stride, lo, hi)``.  (Strides of slices are nested: one or two values of each have to be tried.)"""
+    spans = sorted(spans, reverse=True)
+    tries = 10000
+
+    def solve(k, rest, zero):
+        nonlocal tries
+        if k == len(spans):
+            return rest == 0 and not zero
+        st, lo, hi = spans[k]
+        least, most = (sum(q * span[i] for q, *span in spans[k + 1 :]) for i in (0, 1))
+        for t in range(max(lo, -((most - rest) // st)), min(hi, (rest - least) // st) + 1):
+            tries -= 1
+            if tries < 0 or solve(k + 1, rest - st * t, zero and t == 0):  # (strides that need so many are taken to share)
+                return True
+        return False
+
+    return solve(0, distance, other_than_zero)
+
+
 def _share(a, b):
-    """Whether ``a`` and ``b`` have a byte in common: is there a solution of ``sum stride_k t_k = distance`` with every ``t_k``, a difference of
-    two indices, in its range?  (Strides of slices are nested: one or two values of each have to be tried.)"""
+    """Whether ``a`` and ``b`` have a byte in common."""
     spans = {}
     for t, lo, hi in ((a, 0, 1), (b, -1, 0)):
         for st, n in (*zip((st * t.element_size() for st in t.stride()), t.shape), (1, t.element_size())):
@@ -69,27 +89,21 @@ def _share(a, b):
                 at = spans.setdefault(st, [0, 0])
                 at[0] += lo * (n - 1)
                 at[1] += hi * (n - 1)
-    spans = sorted(((st, *at) for st, at in spans.items()), reverse=True)
-    tries = 10000
+    return _meet([(st, *at) for st, at in spans.items()], b.data_ptr() - a.data_ptr())
 
-    def solve(k, rest):
-        nonlocal tries
-        if k == len(spans):
-            return rest == 0
-        st, lo, hi = spans[k]
-        least, most = (sum(q * span[i] for q, *span in spans[k + 1 :]) for i in (0, 1))
-        for t in range(max(lo, -((most - rest) // st)), min(hi, (rest - least) // st) + 1):
-            tries -= 1
-            if tries < 0 or solve(k + 1, rest - st * t):  # (strides that need so many are taken to share)
-                return True
-        return False
 
-    return solve(0, b.data_ptr() - a.data_ptr())
+def _overlaps_itself(t):
+    """Whether two entries of ``t`` have the same place in memory (an expanded axis, windows that overlap)."""
+    axes = [(st, n) for st, n in zip(t.stride(), t.shape) if n > 1]
+    strides = [st for st, _ in axes]
+    return t.numel() > 0 and (0 in strides or len(set(strides)) < len(strides) or _meet([(st, 1 - n, n - 1) for st, n in axes], 0, True))
 
 
 def _refuse_shared(grads, copies, what):
-    """Tensors that are scaled as a copy are written back whole: raise where one shares memory with another tensor.  (Those that are
-    scaled where they are are compared by the library.)"""
+    """Tensors that are scaled as a copy are written back whole: raise where one shares memory with another tensor, or two of its own entries do.  (Those
+    that are scaled where they are are compared by the library.)"""
+    if any(g is not c and _overlaps_itself(g) for g, c in zip(grads, copies)):
+        raise RuntimeError(f"{what}: two entries of a gradient share memory")
     held = sorted(((*_extent(g), g, g is not c) for g, c in zip(grads, copies) if g.numel()), key=lambda e: e[0])
     near = []  # that reach beyond the first byte of the one at hand
     for lo, hi, g, copied in held:
