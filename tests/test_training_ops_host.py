@@ -264,3 +264,25 @@ def test_gradients_that_overlap_themselves_are_found_exactly():
     for bad in (torch.zeros(1).expand(5), torch.zeros(3, 1).expand(3, 4), base.as_strided((3, 3), (1, 1)), base.as_strided((4, 4), (2, 1))):
         with pytest.raises(RuntimeError, match="share memory"):
             _refuse_shared([torch.zeros(3), bad], [torch.zeros(3), bad.contiguous()], "clip_grad_norm_")
+
+
+def test_c_abi_takes_long_tensors_among_many(lib):
+    """The length of one tensor is not limited by how many others there are; all of a launch together by what 32 bits count.  (Nothing is launched: two of the tensors
+    share memory, which is refused last.)"""
+    n, long = 40_000, 1 << 30
+    ts = [((1 << 20) + 64 * i, 4, 0) for i in range(n)] + [(1 << 30, long, 0), (1 << 40, long, 3), (1 << 40, long, 3)]
+
+    def clip(ts):
+        n, src, numel, dtype = _lists(ts)
+        rc = lib.shtb200_clip_grads(n, src, src, numel, dtype, 0, 1.0, 1 << 16, 1 << 16, 1 << 30, None)
+        return rc, lib.shtb200_last_error()
+
+    rc, why = clip(ts)
+    assert rc == -1 and b"share memory" in why
+    rc, why = clip([((i + 1) << 40, 1 << 36, 0) for i in range(300)])  # 2.5e9 units
+    assert rc == -1 and b"too many entries" in why
+    rc, why = clip([(1 << 20, (1 << 44) + 1, 0)])
+    assert rc == -1 and b"length" in why
+    # as many units, but in two launches
+    rc, why = clip([((i + 1) << 40, 1 << 34, 0) for i in range(1400)] + [(1 << 40, 4, 0)])
+    assert rc == -1 and b"share memory" in why

@@ -15,6 +15,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 namespace shtb200 {
@@ -41,6 +42,9 @@ template <int N> struct Table {
 static_assert(sizeof(Table<kMaxTensors>) + 64 <= 32764, "kernel arguments");
 
 __host__ __device__ constexpr int unit_values(int dtype) { return dtype == SHTB200_BF16 || dtype == SHTB200_F16 ? kUnitBytes / 2 : kUnitBytes / 4; }
+
+constexpr long long values_of(long long numel, int dtype) { return numel * (dtype == SHTB200_C64 ? 2 : 1); }
+constexpr long long units_of(long long numel, int dtype) { return (values_of(numel, dtype) + unit_values(dtype) - 1) / unit_values(dtype); }
 
 template <typename T> struct Pack {  // 16 bytes of values
     static constexpr int n = 16 / sizeof(T);
@@ -249,10 +253,18 @@ int check_tensors(int count, const void *const *src, void *const *dst, const lon
         bool written;
     };
     std::vector<Range> r;
+    long long units = 0;  // of a launch: they are counted in 32 bits, with room for a step beyond the last
+    int in_launch = 0;
     for (int i = 0; i < count; ++i) {
         if (dtype[i] < SHTB200_F32 || dtype[i] > SHTB200_C64) return fail(SHTB200_EINVAL, "unknown element type");
-        if (numel[i] < 0 || numel[i] > (1LL << 40) / std::max(count, 1)) return fail(SHTB200_EINVAL, "bad tensor length");
+        if (numel[i] < 0 || numel[i] > (1LL << 44)) return fail(SHTB200_EINVAL, "bad tensor length");
         if (numel[i] == 0) continue;
+        if (in_launch++ == kMaxTensors) {
+            units = 0;
+            in_launch = 1;
+        }
+        units += units_of(numel[i], dtype[i]);
+        if (units > INT_MAX - kMaxBlocks) return fail(SHTB200_EINVAL, "too many entries: at most 2^31 pieces of 32 KB in " + std::to_string(kMaxTensors) + " tensors");
         if (!src[i] || (dst && !dst[i])) return fail(SHTB200_EINVAL, "null pointer");
         const size_t es = std::min<size_t>(bytes_of(dtype[i]), 4), bytes = bytes_of(dtype[i]) * (size_t)numel[i];
         if ((uintptr_t)src[i] % es || (dst && (uintptr_t)dst[i] % es)) return fail(SHTB200_EINVAL, "a tensor is not aligned to its element type");
@@ -309,9 +321,9 @@ struct List {
             const int i = index[(size_t)launch * kMaxTensors + k];
             t->src[k] = src[i];
             t->dst[k] = dst ? dst[i] : nullptr;
-            t->n[k] = numel[i] * (dtype[i] == SHTB200_C64 ? 2 : 1);
+            t->n[k] = values_of(numel[i], dtype[i]);
             t->dtype[k] = (unsigned char)dtype[i];
-            t->first[k + 1] = t->first[k] + (int)((t->n[k] + unit_values(dtype[i]) - 1) / unit_values(dtype[i]));
+            t->first[k + 1] = t->first[k] + (int)units_of(numel[i], dtype[i]);
         }
     }
 };
