@@ -179,7 +179,7 @@ int shtb200_group_norm_backward(const shtb200_group_norm_desc *desc, const void 
  * Norm over all entries of `count` tensors of any of the element types (SHTB200_NORM_L2: root of the sum of |g|^2, in float64;
  * SHTB200_NORM_INF: largest |g|), written to *norm_dev; 0 for no entries.  The arrays of pointers, lengths (entries) and types are host
  * memory and are read before the call returns.  shtb200_clip_grads then writes dst = src * min(1, max_norm / (norm + 1e-6)); dst[i]
- * may be src[i], otherwise no two of the buffers may share memory where one is written (SHTB200_EINVAL).  Where nothing is to be clipped, tensors in
+ * may be src[i], otherwise no two of the buffers, the norm among them, may share memory where one is written (SHTB200_EINVAL).  Where nothing is to be clipped, tensors in
  * place are not touched.  A norm that is not finite goes the same way: inf gives the factor 0, NaN gives NaN.
  * Workspace: shtb200_grad_norm_workspace_bytes(count), 8-byte aligned.  Current device, no synchronisation, may be captured.
  */

@@ -313,3 +313,16 @@ def test_expanded_gradients():
         with pytest.raises(RuntimeError, match="share memory"):
             clip()
         assert torch.equal(a, old) and float(one) == 2.0
+
+
+def test_norm_that_is_a_gradient_itself():
+    """The norm of a single scalar parameter is its gradient: refused as it stands, taken as a copy."""
+    import torch_harmonics_b200 as th
+
+    p = torch.nn.Parameter(torch.zeros((), device="cuda"))
+    p.grad = torch.full((), 3.0, device="cuda")
+    with pytest.raises(RuntimeError, match="share memory"):
+        th.clip_grads_with_norm_(p, 1.0, p.grad)
+    assert float(p.grad) == 3.0
+    th.clip_grads_with_norm_(p, 1.0, p.grad.clone())
+    _clipped_right([p.grad], [torch.full((), 3.0, device="cuda")], 3.0, 1.0)

@@ -286,3 +286,15 @@ def test_c_abi_takes_long_tensors_among_many(lib):
     # as many units, but in two launches
     rc, why = clip([((i + 1) << 40, 1 << 34, 0) for i in range(1400)] + [(1 << 40, 4, 0)])
     assert rc == -1 and b"share memory" in why
+
+
+def test_c_abi_refuses_a_norm_inside_the_tensors(lib):
+    """Every block reads the norm while others scale: it may not lie in what is written, nor, where it is written itself, in what is read."""
+    at, other, ws = 1 << 20, 1 << 21, 1 << 16
+    n, src, numel, dtype = _lists([(at, 100, 0), (at + 4096, 100, 3)])
+    away = (ctypes.c_uint64 * n)(other, other + 4096)
+    for norm in (at, at + 396, at + 4096, at + 4096 + 796):
+        assert lib.shtb200_scale_grads(n, src, src, numel, dtype, 1.0, norm, None) == -1 and b"share memory" in lib.shtb200_last_error()
+        assert lib.shtb200_clip_grads(n, src, src, numel, dtype, 0, 1.0, norm, ws, 1 << 30, None) == -1 and b"share memory" in lib.shtb200_last_error()
+        assert lib.shtb200_clip_grads(n, src, away, numel, dtype, 0, 1.0, norm, ws, 1 << 30, None) == -1
+        assert lib.shtb200_scale_grads(n, src, away, numel, dtype, 1.0, norm + (other - at), None) == -1

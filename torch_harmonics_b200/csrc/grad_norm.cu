@@ -246,7 +246,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) scale_kernel(const __g
 
 size_t bytes_of(int dtype) { return dtype == SHTB200_C64 ? 8 : dtype == SHTB200_F32 ? 4 : 2; }
 
-int check_tensors(int count, const void *const *src, void *const *dst, const long long *numel, const int *dtype) {
+// norm: read by every block, and in a clipping written by one
+int check_tensors(int count, const void *const *src, void *const *dst, const long long *numel, const int *dtype, const float *norm, bool norm_written) {
     if (count < 0 || (count > 0 && (!src || !numel || !dtype))) return fail(SHTB200_EINVAL, "bad tensor list");
     struct Range {
         uintptr_t lo, hi;
@@ -273,11 +274,12 @@ int check_tensors(int count, const void *const *src, void *const *dst, const lon
             if (src[i] != dst[i]) r.push_back({(uintptr_t)src[i], (uintptr_t)src[i] + bytes, false});
         }
     }
-    // Two tensors that share memory would be scaled twice, in no fixed order.
+    // Two tensors that share memory would be scaled twice, in no fixed order, and a norm among them read before or after it is scaled.
+    if (dst) r.push_back({(uintptr_t)norm, (uintptr_t)norm + sizeof(float), norm_written});
     std::sort(r.begin(), r.end(), [](const Range &a, const Range &b) { return a.lo < b.lo; });
     uintptr_t end_any = 0, end_written = 0;
     for (const Range &x : r) {
-        if (x.lo < (x.written ? end_any : end_written)) return fail(SHTB200_EINVAL, "two of the tensors to be scaled share memory");
+        if (x.lo < (x.written ? end_any : end_written)) return fail(SHTB200_EINVAL, "two of the tensors to be scaled, or one and the norm, share memory");
         end_any = std::max(end_any, x.hi);
         if (x.written) end_written = std::max(end_written, x.hi);
     }
@@ -380,7 +382,7 @@ int check_norm(int count, int kind, const float *norm, const void *ws, size_t ws
 
 int grad_norm(int count, const void *const *src, const long long *numel, const int *dtype, int kind, float *norm, void *ws, size_t ws_bytes, cudaStream_t st) {
     int rc = check_norm(count, kind, norm, ws, ws_bytes);
-    if (rc || (rc = check_tensors(count, src, nullptr, numel, dtype))) return rc;
+    if (rc || (rc = check_tensors(count, src, nullptr, numel, dtype, norm, true))) return rc;
     double *part = reinterpret_cast<double *>(ws);
     int nparts = 0;
     if ((rc = launch_partials(make_list(count, src, nullptr, numel, dtype), kind, part, &nparts, st))) return rc;
@@ -391,7 +393,7 @@ int clip_grads(int count, const void *const *src, void *const *dst, const long l
                cudaStream_t st) {
     if (!(max_norm >= 0.f)) return fail(SHTB200_EINVAL, "max_norm must be >= 0");
     int rc = check_norm(count, kind, norm, ws, ws_bytes);
-    if (rc || (rc = check_tensors(count, src, dst, numel, dtype))) return rc;
+    if (rc || (rc = check_tensors(count, src, dst, numel, dtype, norm, true))) return rc;
     const List l = make_list(count, src, dst, numel, dtype);
     double *part = reinterpret_cast<double *>(ws);
     int nparts = 0;
@@ -402,7 +404,7 @@ int clip_grads(int count, const void *const *src, void *const *dst, const long l
 int scale_grads(int count, const void *const *src, void *const *dst, const long long *numel, const int *dtype, float max_norm, const float *norm, cudaStream_t st) {
     if (!(max_norm >= 0.f)) return fail(SHTB200_EINVAL, "max_norm must be >= 0");
     if (!norm) return fail(SHTB200_EINVAL, "null pointer");
-    int rc = check_tensors(count, src, dst, numel, dtype);
+    int rc = check_tensors(count, src, dst, numel, dtype, norm, false);
     if (rc) return rc;
     return launch_scale(make_list(count, src, dst, numel, dtype), SHTB200_NORM_L2, nullptr, 0, max_norm, const_cast<float *>(norm), st);
 }
