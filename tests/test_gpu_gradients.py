@@ -326,3 +326,15 @@ def test_norm_that_is_a_gradient_itself():
     assert float(p.grad) == 3.0
     th.clip_grads_with_norm_(p, 1.0, p.grad.clone())
     _clipped_right([p.grad], [torch.full((), 3.0, device="cuda")], 3.0, 1.0)
+
+
+def test_norm_with_a_lazy_minus_sign():
+    import torch_harmonics_b200 as th
+
+    norm = torch.view_as_complex(torch.tensor([0.5, -8.0], device="cuda")).conj().imag  # 8, held as -8
+    assert norm.is_neg() and norm.is_contiguous()
+    (g,) = _tensors([((100,), F32)])
+    p = torch.nn.Parameter(torch.zeros(100, device="cuda"))
+    p.grad = g.clone()
+    th.clip_grads_with_norm_(p, 2.0, norm)
+    _clipped_right([p.grad], [g], 8.0, 2.0)

@@ -243,7 +243,7 @@ def clip_grads_with_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]
     ls = _List(grads, "clip_grads_with_norm_")
     if total_norm.numel() != 1 or total_norm.device != grads[0].device:
         raise RuntimeError(f"clip_grads_with_norm_: expected total_norm as a scalar on {grads[0].device}, got shape {tuple(total_norm.shape)} on {total_norm.device}")
-    _clip_in_place(grads, ls, max_norm, _lib.NORM_L2, "clip_grads_with_norm_", total_norm.to(torch.float32).contiguous())
+    _clip_in_place(grads, ls, max_norm, _lib.NORM_L2, "clip_grads_with_norm_", _lib.dense(total_norm.to(torch.float32)))
 
 
 @torch.no_grad()
