@@ -686,3 +686,41 @@ def test_lazy_minus_sign_keeps_the_layout():
     with torch.no_grad():
         y = m(n)
     assert y.is_contiguous(memory_format=torch.channels_last) and torch.equal(y, m(-x))
+
+
+@pytest.mark.parametrize("fmt", ["planes", "last", "strided"])
+@pytest.mark.parametrize("affine,weighted", [(True, True), (False, True), (True, False)])
+def test_traces_into_one_graph(affine, weighted, fmt):
+    """Between transforms under torch.compile(fullgraph=True): the same values and gradients as eager, with and without parameters and weights."""
+    import torch_harmonics_b200 as th
+    from torch_harmonics_b200.normalization import _group_norm, _group_norm_backward
+
+    torch._dynamo.reset()  # (one code object for all cases: its compilations are counted together)
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        sht, isht = th.RealSHT(33, 64, grid="equiangular").cuda(), th.InverseRealSHT(33, 64, grid="equiangular").cuda()
+    m = _module(2, 6, 33, 64, activation="gelu", affine=affine, weighted=weighted)
+    _parameters(m)
+    x = torch.randn(2, 6, 33, 64, device="cuda")
+    leaves = [x.requires_grad_(True), *m.parameters()]
+
+    def f(t):
+        t = isht(sht(t)) * 2
+        t = t.contiguous(memory_format=torch.channels_last) if fmt == "last" else torch.cat([t, t], -1)[..., 1:65] if fmt == "strided" else t
+        return isht(sht(m(t).contiguous())).square()
+
+    want = f(x)
+    grads = torch.autograd.grad(want.sum(), leaves)
+    got = torch.compile(f, fullgraph=True, backend="aot_eager")(x)
+    assert torch.equal(got, want)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got.sum(), leaves), grads))
+    with torch.no_grad():
+        assert torch.equal(torch.compile(f, fullgraph=True, backend="aot_eager")(x), want)
+    t = x.detach()
+    t = t.contiguous(memory_format=torch.channels_last) if fmt == "last" else torch.cat([t, t], -1)[..., 1:65] if fmt == "strided" else t
+    how = (m.weight, m.bias, m.lat_weights, 2, m.eps, "gelu")
+    checks = ("test_schema", "test_faketensor", "test_autograd_registration")
+    torch.library.opcheck(_group_norm, (t.clone().requires_grad_(True), *how), test_utils=checks)
+    y, stats = _group_norm(t, *how)
+    assert torch.equal(y, m(t)) and y.stride() == m(t).stride()
+    torch.library.opcheck(_group_norm_backward, (torch.randn_like(y), t, *how[:3], stats, *how[3:], [True, affine, False]), test_utils=checks[:2])

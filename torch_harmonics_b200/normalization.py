@@ -5,8 +5,8 @@ latitude quadrature weights of the grid (``QuadratureS2``), so that the many gri
 their area.  ``weighted=False`` gives the plain averages over grid points of ordinary group normalisation.
 """
 
-import ctypes
-from typing import Optional, Tuple
+import functools
+from typing import List, Optional, Tuple
 
 import torch
 import torch.nn as nn
@@ -33,14 +33,36 @@ def _aligned(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _run(module, x, weight, bias, lat, keep):
+def _call(batch, channels, groups, nlat, nlon, dtype, param_dtype, channels_last, activation, eps):
+    """(descriptor, workspace bytes forward, backward): shapes and types only."""
+    desc = _lib.GroupNormDesc(batch, channels, groups, nlat, nlon, _DTYPES[dtype], _DTYPES[param_dtype], int(channels_last), _lib.ACTIVATIONS[activation], eps)
+    ws = [_lib.load().shtb200_group_norm_workspace_bytes(desc, i) for i in (0, 1)]
+    if ws[0] == 0:
+        _lib.check(-1, "shtb200_group_norm_workspace_bytes")
+    return desc, *ws
+
+
+def _stats_bytes(batch, groups):
+    return (16 * batch * groups + 255) // 256 * 256
+
+
+def _taken(x):
+    """``x`` as the kernels read it: planes or channels last, without a lazy sign, aligned."""
+    if x.is_neg():
+        x = x.resolve_neg()
+    if not (x.is_contiguous() or x.is_contiguous(memory_format=torch.channels_last)):
+        x = x.contiguous()
+    return _aligned(x)
+
+
+def _run(call, x, weight, bias, lat, keep):
     """y and (with ``keep``) what the backward pass needs, for a dense ``x``."""
-    desc, ws_bytes, _ = module._call(x, weight)
-    batch, dev = x.shape[0], x.device
+    desc, ws_bytes, _ = call
+    dev = x.device
     y = torch.empty_like(x)
-    stats_bytes = (16 * batch * module.num_groups + 255) // 256 * 256
+    stats_bytes = _stats_bytes(desc.batch, desc.groups)
     stats = torch.empty(stats_bytes if keep else stats_bytes + ws_bytes, dtype=torch.uint8, device=dev)
-    if batch == 0:
+    if desc.batch == 0:
         return y, stats
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if keep else None
     at = stats.data_ptr()
@@ -53,12 +75,33 @@ def _run(module, x, weight, bias, lat, keep):
     return y, stats
 
 
+def _run_backward(call, dy, x, weight, bias, lat, stats, need):
+    """dx, dweight, dbias, ``None`` where ``need`` says so."""
+    desc, _, ws_bytes = call
+    new = torch.empty_like if desc.batch else torch.zeros_like
+    dx = torch.empty_like(x) if need[0] else None
+    dw = new(weight) if need[1] else None
+    db = new(bias) if need[2] else None
+    if desc.batch == 0:
+        return dx, dw, db
+    # the gradient comes in any layout (an expanded scalar, for a sum): the kernel reads it in the layout of x
+    dy = _aligned(_lib.dense(dy) if not desc.channels_last else dy.resolve_neg().contiguous(memory_format=torch.channels_last))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+    with _lib.on_device(x.device.index) as stream:
+        rc = _lib.load().shtb200_group_norm_backward(
+            desc, dy.data_ptr(), x.data_ptr(), _ptr(lat), _ptr(weight), _ptr(bias), stats.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(), ws_bytes, stream
+        )
+    if rc != 0:
+        _lib.check(rc, "shtb200_group_norm_backward")
+    return dx, dw, db
+
+
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, lat, module):
-        y, stats = _run(module, x, weight, bias, lat, True)
+    def forward(ctx, x, weight, bias, lat, call):
+        y, stats = _run(call, x, weight, bias, lat, True)
         ctx.save_for_backward(x, weight, bias, lat, stats)
-        ctx.call = module._call(x, weight)
+        ctx.call = call
         return y
 
     @staticmethod
@@ -69,27 +112,71 @@ class _GroupNorm(torch.autograd.Function):
 
 def _gradients(ctx, dy):
     x, weight, bias, lat, stats = ctx.saved_tensors
-    desc, _, ws_bytes = ctx.call
-    new = torch.empty_like if x.shape[0] else torch.zeros_like
-    need = ctx.needs_input_grad
-    dx = torch.empty_like(x) if need[0] else None
-    dw = new(weight) if need[1] else None
-    db = new(bias) if need[2] else None
-    if x.shape[0] == 0:
-        return dx, dw, db, None, None
-    # the gradient comes in any layout (an expanded scalar, for a sum): the kernel reads it in the layout of x
-    dy = _aligned(_lib.dense(dy) if not desc.channels_last else dy.resolve_neg().contiguous(memory_format=torch.channels_last))
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
-    with _lib.on_device(x.device.index) as stream:
-        rc = _lib.load().shtb200_group_norm_backward(
-            desc, dy.data_ptr(), x.data_ptr(), _ptr(lat), _ptr(weight), _ptr(bias), stats.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(), ws_bytes, stream
-        )
-    if rc != 0:
-        _lib.check(rc, "shtb200_group_norm_backward")
-    return dx, dw, db, None, None
+    return *_run_backward(ctx.call, dy, x, weight, bias, lat, stats, ctx.needs_input_grad), None, None
 
 
 _guarded_gradients = once_differentiable(_gradients)
+
+
+# Where torch.compile traces, the call is a custom operator (as the transforms are), so that a network stays one graph.  Eager calls take the function
+# above instead, which is half the host time of such an operator.
+_traced_call = functools.lru_cache(maxsize=256)(_call)
+
+
+def _call_of(x, weight, groups, eps, activation):
+    return _traced_call(*x.shape[:2], groups, *x.shape[2:], x.dtype, torch.float32 if weight is None else weight.dtype, not x.is_contiguous(), activation, eps)
+
+
+def _dense(t):
+    return None if t is None else _lib.dense(t)
+
+
+@torch.library.custom_op("shtb200::group_norm", mutates_args=(), device_types="cuda")
+def _group_norm(
+    x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], lat: Optional[torch.Tensor], groups: int, eps: float, activation: Optional[str]
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    x = _taken(x)
+    return _run(_call_of(x, weight, groups, eps, activation), x, _dense(weight), _dense(bias), _dense(lat), True)
+
+
+@torch.library.custom_op("shtb200::group_norm_backward", mutates_args=(), device_types="cuda")
+def _group_norm_backward(
+    dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], lat: Optional[torch.Tensor], stats: torch.Tensor,
+    groups: int, eps: float, activation: Optional[str], need: List[bool],
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:  # fmt: skip
+    x, weight, bias = _taken(x), _dense(weight), _dense(bias)
+    out = _run_backward(_call_of(x, weight, groups, eps, activation), dy, x, weight, bias, _dense(lat), stats, need)
+    return tuple(x.new_empty(0) if t is None else t for t in out)
+
+
+def _fake_like(x):
+    kept = x.is_contiguous() or x.is_contiguous(memory_format=torch.channels_last)
+    return torch.empty_like(x, memory_format=torch.preserve_format if kept else torch.contiguous_format)
+
+
+@_group_norm.register_fake
+def _(x, weight, bias, lat, groups, eps, activation):
+    return _fake_like(x), x.new_empty(_stats_bytes(x.shape[0], groups), dtype=torch.uint8)
+
+
+@_group_norm_backward.register_fake
+def _(dy, x, weight, bias, lat, stats, groups, eps, activation, need):
+    return tuple(make(t) if n else x.new_empty(0) for t, n, make in zip((x, weight, bias), need, (_fake_like, *[lambda p: p.new_empty(p.shape)] * 2)))
+
+
+def _setup(ctx, inputs, output):
+    x, weight, bias, lat, *ctx.how = inputs
+    ctx.save_for_backward(x, weight, bias, lat, output[1])
+
+
+def _traced_gradients(ctx, dy, _):
+    x, weight, bias, lat, stats = ctx.saved_tensors
+    need = [bool(n) for n in ctx.needs_input_grad[:3]]
+    grads = _group_norm_backward(dy, x, weight, bias, lat, stats, *ctx.how, need)
+    return *(g if n else None for g, n in zip(grads, need)), None, None, None, None
+
+
+_group_norm.register_autograd(_traced_gradients, setup_context=_setup)
 
 
 class GroupNormS2(nn.Module):
@@ -204,19 +291,12 @@ class GroupNormS2(nn.Module):
         return _lib.dense(lat)
 
     def _call(self, x, weight):
-        """(descriptor, workspace bytes forward, backward) of a call on ``x``: shapes and types only."""
         param = torch.float32 if weight is None else weight.dtype
         cl = not x.is_contiguous()
         key = (x.shape[0], x.dtype, param, cl, self.eps, self.activation)
         call = self._calls.get(key)
         if call is None:
-            desc = _lib.GroupNormDesc(
-                x.shape[0], self.num_channels, self.num_groups, self.nlat, self.nlon, _DTYPES[x.dtype], _DTYPES[param], int(cl), _lib.ACTIVATIONS[self.activation], self.eps
-            )
-            ws = [_lib.load().shtb200_group_norm_workspace_bytes(desc, i) for i in (0, 1)]
-            if ws[0] == 0:
-                _lib.check(-1, "shtb200_group_norm_workspace_bytes")
-            call = self._calls[key] = (desc, *ws)
+            call = self._calls[key] = _call(x.shape[0], self.num_channels, self.num_groups, self.nlat, self.nlon, x.dtype, param, cl, self.activation, self.eps)
         return call
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
@@ -230,11 +310,10 @@ class GroupNormS2(nn.Module):
             raise RuntimeError(f"Expected shape (batch, {self.num_channels}, {self.nlat}, {self.nlon}), got {tuple(x.shape)}")
         weight, bias = self._affine(x.device)
         lat = self._lat(x.device)
-        if x.is_neg():
-            x = x.resolve_neg()
-        if not (x.is_contiguous() or x.is_contiguous(memory_format=torch.channels_last)):
-            x = x.contiguous()
-        x = _aligned(x)
+        if torch.compiler.is_compiling():
+            return _group_norm(x, weight, bias, lat, self.num_groups, self.eps, self.activation)[0]
+        x = _taken(x)
+        call = self._call(x, weight)
         if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and (weight.requires_grad or bias.requires_grad))):
-            return _GroupNorm.apply(x, weight, bias, lat, self)
-        return _run(self, x, weight, bias, lat, False)[0]
+            return _GroupNorm.apply(x, weight, bias, lat, call)
+        return _run(call, x, weight, bias, lat, False)[0]
