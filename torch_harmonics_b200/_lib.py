@@ -8,6 +8,8 @@ import ctypes
 import os
 import threading
 
+import torch
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libshtb200.so")
 
@@ -41,6 +43,8 @@ class ShtLibraryError(RuntimeError):
 def load():
     """Load the library once; raise ``ShtLibraryError`` if it has not been built."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -128,8 +132,6 @@ class on_device:
         self.index = index
 
     def __enter__(self):
-        import torch
-
         self.previous = torch._C._cuda_getDevice()
         if self.previous != self.index:
             torch.cuda.set_device(self.index)
@@ -137,8 +139,6 @@ class on_device:
 
     def __exit__(self, *exc):
         if self.previous != self.index:
-            import torch
-
             torch.cuda.set_device(self.previous)
 
 
@@ -167,8 +167,6 @@ def rows_pieces_supported(nlon, nmodes, grid_pieces, mode_pieces):
 
 def spectral_conv(analysis, synthesis, x, weight, y, batch, cin, cout, groups, stream):
     """SHT -> per-degree channel mixing -> inverse SHT on device tensors (``shtb200_spectral_conv``)."""
-    import torch
-
     lib = load()
     nbytes = lib.shtb200_spectral_conv_workspace_bytes(analysis.handle, synthesis.handle, batch, cin, cout, groups)
     if nbytes == 0:
@@ -192,8 +190,6 @@ class Plan:
     def __init__(self, kind, nlat, nlon, lmax, mmax, table_f32_cuda, engine="auto", orders=None):
         """``orders = (m_first, m_count)`` builds a plan for that window of orders from a table that holds them only
         (``shtb200_plan_create_orders``); such a plan serves :meth:`legendre` alone."""
-        import torch
-
         lib = load()
         if not table_f32_cuda.is_cuda or table_f32_cuda.dtype != torch.float32 or not table_f32_cuda.is_contiguous():
             raise ShtLibraryError("the Legendre table must be a contiguous float32 CUDA tensor")

@@ -33,6 +33,11 @@ def _aligned(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _dense(t):
+    """``_lib.dense`` of a real tensor or none, at next to no cost where there is nothing to do."""
+    return t if t is None or t.is_contiguous() and not t.is_neg() else _lib.dense(t)
+
+
 def _call(batch, channels, groups, nlat, nlon, dtype, param_dtype, channels_last, activation, eps):
     """(descriptor, workspace bytes forward, backward): shapes and types only."""
     desc = _lib.GroupNormDesc(batch, channels, groups, nlat, nlon, _DTYPES[dtype], _DTYPES[param_dtype], int(channels_last), _lib.ACTIVATIONS[activation], eps)
@@ -125,10 +130,6 @@ _traced_call = functools.lru_cache(maxsize=256)(_call)
 
 def _call_of(x, weight, groups, eps, activation):
     return _traced_call(*x.shape[:2], groups, *x.shape[2:], x.dtype, torch.float32 if weight is None else weight.dtype, not x.is_contiguous(), activation, eps)
-
-
-def _dense(t):
-    return None if t is None else _lib.dense(t)
 
 
 @torch.library.custom_op("shtb200::group_norm", mutates_args=(), device_types="cuda")
@@ -260,8 +261,8 @@ class GroupNormS2(nn.Module):
         state = super().__getstate__() if hasattr(super(), "__getstate__") else self.__dict__
         return {**state, "_calls": {}}
 
-    def _affine(self, device):
-        """``weight`` and ``bias`` as the kernels read them.  They may have been replaced since the module was made."""
+    def _affine(self, device, traced=False):
+        """``weight`` and ``bias`` as the kernels read them (``traced``: as they are).  They may have been replaced since the module was made."""
         weight, bias = self.weight, self.bias
         if weight is None and bias is None:
             return None, None
@@ -273,11 +274,13 @@ class GroupNormS2(nn.Module):
             raise TypeError(f"GroupNormS2: weight and bias must both be float32, bfloat16 or float16, got {weight.dtype} and {bias.dtype}")
         if weight.shape != (self.num_channels,) or bias.shape != (self.num_channels,):
             raise RuntimeError(f"GroupNormS2: expected weight and bias of shape ({self.num_channels},), got {tuple(weight.shape)} and {tuple(bias.shape)}")
-        return _lib.dense(weight), _lib.dense(bias)  # (one value expanded to all channels is a copy here, and its gradient a sum)
+        if traced:
+            return weight, bias
+        return _dense(weight), _dense(bias)  # (one value expanded to all channels is a copy here, and its gradient a sum)
 
-    def _lat(self, device):
+    def _lat(self, device, traced=False):
         """``lat_weights`` as the kernels read them.  They may have been replaced too (by a mask of rows, for instance)."""
-        lat = self.lat_weights
+        lat = self._buffers["lat_weights"] if "lat_weights" in self._buffers else self.lat_weights  # (the attribute takes five times as long)
         if lat is None:
             return None
         if lat.device != device:
@@ -288,7 +291,7 @@ class GroupNormS2(nn.Module):
             raise RuntimeError(f"GroupNormS2: expected lat_weights of shape ({self.nlat},), got {tuple(lat.shape)}")
         if lat.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("GroupNormS2: lat_weights get no gradient, they must not require one")
-        return _lib.dense(lat)
+        return lat if traced else _dense(lat)
 
     def _call(self, x, weight):
         param = torch.float32 if weight is None else weight.dtype
@@ -308,9 +311,10 @@ class GroupNormS2(nn.Module):
             raise RuntimeError(f"Expected tensor with 4 dimensions but got {x.dim()} instead")
         if x.shape[1:] != (self.num_channels, self.nlat, self.nlon):
             raise RuntimeError(f"Expected shape (batch, {self.num_channels}, {self.nlat}, {self.nlon}), got {tuple(x.shape)}")
-        weight, bias = self._affine(x.device)
-        lat = self._lat(x.device)
-        if torch.compiler.is_compiling():
+        traced, device = torch.compiler.is_compiling(), x.device
+        weight, bias = self._affine(device, traced)
+        lat = self._lat(device, traced)
+        if traced:
             return _group_norm(x, weight, bias, lat, self.num_groups, self.eps, self.activation)[0]
         x = _taken(x)
         call = self._call(x, weight)
