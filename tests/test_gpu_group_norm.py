@@ -724,3 +724,22 @@ def test_traces_into_one_graph(affine, weighted, fmt):
     y, stats = _group_norm(t, *how)
     assert torch.equal(y, m(t)) and y.stride() == m(t).stride()
     torch.library.opcheck(_group_norm_backward, (torch.randn_like(y), t, *how[:3], stats, *how[3:], [True, affine, False]), test_utils=checks[:2])
+
+
+@pytest.mark.parametrize("fmt", ["planes", "last"])
+@pytest.mark.parametrize("act", [None, "silu", "gelu"])
+@pytest.mark.parametrize("shape", [(1, 16, 4, 721, 1440), (2, 32, 8, 256, 512)], ids=lambda s: "x".join(map(str, s)))
+def test_errors_in_the_mean_square(shape, act, fmt):
+    """float32, where the bound for single values above leaves room for several bits: root-mean-square errors relative to the results'.
+
+    A value of z has three roundings and the errors of m and r, four more at most: 7 x 2^-24.  Activations and slopes add a fit and two approximate
+    instructions, 2^-22 each: 7 x 2^-24 + 3 x 2^-22 = 1.2 x 2^-20, of single values, whose mean square is a third of it (uniform): 2^-20 is left for y and dx.
+    Sums over a channel of terms of either sign grow like their errors, with n terms by sqrt(n).  To them add the roundings of a thread's running sum: of 2,000
+    terms, sqrt(2000) x 0.2 x 2^-24 = 2^-20.8 of its own size.  2^-19 for dweight and dbias."""
+    B, C, G, H, W = shape
+    m = _module(G, C, H, W, activation=act)
+    _parameters(m)
+    x, dy = _inputs((B, C, H, W), torch.float32, fmt)
+    for name, o, e, bound in zip(("y", "dx", "dweight", "dbias"), _step(m, x, dy), _exact(m, x, dy)[0], (2.0**-20, 2.0**-20, 2.0**-19, 2.0**-19)):
+        off = float((o.double() - e).norm() / e.norm())
+        assert off <= bound, f"{name}: {off:.2e}"
