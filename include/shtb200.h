@@ -160,7 +160,7 @@ enum shtb200_norm { SHTB200_NORM_L2 = 0, SHTB200_NORM_INF = 1 };
  * channels_last = 0: [batch, channels, nlat, nlon]; 1: [batch, nlat, nlon, channels].  Statistics and sums are float32 or wider.
  *   forward : y and stats (16 bytes per (sample, group), 16-byte aligned: what the backward pass needs).
  *   backward: dx, dweight, dbias, each of which may be NULL; the sums over the batch are taken in a fixed order.
- * x and y (dy and dx) may not overlap, and the tensors of a call have the same address modulo 16 (else SHTB200_EINVAL).  Workspace: shtb200_group_norm_workspace_bytes(desc, backward) bytes, 256-byte aligned, 0 for a bad
+ * x and y (dy and dx) may not overlap, and the tensors of a call have the same address modulo 16, a multiple of their element size (else SHTB200_EINVAL).  Workspace: shtb200_group_norm_workspace_bytes(desc, backward) bytes, 256-byte aligned, 0 for a bad
  * descriptor.  Runs on the calling thread's current device; no synchronisation; may be captured.
  */
 #define SHTB200_GROUP_NORM_MAX_CHANNELS 4096

@@ -298,3 +298,21 @@ def test_c_abi_refuses_a_norm_inside_the_tensors(lib):
         assert lib.shtb200_clip_grads(n, src, src, numel, dtype, 0, 1.0, norm, ws, 1 << 30, None) == -1 and b"share memory" in lib.shtb200_last_error()
         assert lib.shtb200_clip_grads(n, src, away, numel, dtype, 0, 1.0, norm, ws, 1 << 30, None) == -1
         assert lib.shtb200_scale_grads(n, src, away, numel, dtype, 1.0, norm + (other - at), None) == -1
+
+
+def test_c_abi_refuses_values_off_their_alignment(lib):
+    """All fields a byte off alike: no vector would lie on a 16-byte boundary, wherever it begins."""
+    desc = dict(batch=1, channels=4, groups=2, nlat=8, nlon=16, dtype=0, param_dtype=0, channels_last=0, activation=0, eps=1e-5)
+    at, ws = 4096, 1 << 20
+
+    def forward(x=0, w=0, lat=0, **k):
+        d = _lib.GroupNormDesc(**{**desc, **k})
+        return lib.shtb200_group_norm_forward(d, at + x, at + lat, at + w, None, 2 * at + x, at, ws, 1 << 30, None)
+
+    def backward(x=0, w=0, dw=0, **k):
+        d = _lib.GroupNormDesc(**{**desc, **k})
+        return lib.shtb200_group_norm_backward(d, at + x, 2 * at + x, None, None, at + w, at, 3 * at + x, at + dw, None, ws, 1 << 30, None)
+
+    for rc in (lambda: forward(x=1), lambda: forward(x=2), lambda: forward(x=1, dtype=1), lambda: forward(w=2), lambda: forward(w=1, param_dtype=2), lambda: forward(lat=2),
+               lambda: backward(x=3), lambda: backward(x=1, dtype=2), lambda: backward(w=2), lambda: backward(dw=1), lambda: backward(dw=1, param_dtype=1)):  # fmt: skip
+        assert rc() == -1 and b"aligned to its element type" in lib.shtb200_last_error()

@@ -26,6 +26,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <numeric>
@@ -1419,7 +1420,6 @@ size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
 struct Launch {
     GnArgs a{};
-    bool backward = false;
     size_t part = 0, csum = 0;  // bytes of workspace
     size_t total() const { return part + csum; }
 };
@@ -1432,7 +1432,6 @@ constexpr int kMaxPieces = 4;
 
 Launch geometry(const GroupNormDesc &d, bool backward) {
     Launch l;
-    l.backward = backward;
     GnArgs &a = l.a;
     const int V = 16 / value_bytes(d.dtype);
     a.hw = (long long)d.nlat * d.nlon;
@@ -1557,6 +1556,14 @@ int plan(const GroupNormDesc *d, bool backward, const void *ws, size_t ws_bytes,
     if ((long long)l->a.chunk_px * l->a.cu > (1 << 30) || (long long)l->a.tasks * l->a.pieces > (1 << 30)) return fail(SHTB200_EINVAL, "group norm shape too large");
     return SHTB200_OK;
 }
+// every value lies on a multiple of its size (vectors begin a whole number of values behind the first)
+int check_values(const GroupNormDesc &d, std::initializer_list<const void *> fields, std::initializer_list<const void *> params, const float *lat) {
+    uintptr_t f = 0, p = 0;
+    for (const void *t : fields) f |= (uintptr_t)t;
+    for (const void *t : params) p |= (uintptr_t)t;
+    if (f % value_bytes(d.dtype) || p % value_bytes(d.param_dtype) || (uintptr_t)lat % sizeof(float)) return fail(SHTB200_EINVAL, "a tensor is not aligned to its element type");
+    return SHTB200_OK;
+}
 // vectors are aligned in all tensors or in none
 bool aligned_alike(const void *p, const void *q) { return !p || !q || (((uintptr_t)p ^ (uintptr_t)q) & 15) == 0; }
 
@@ -1574,6 +1581,7 @@ int group_norm_forward(const GroupNormDesc *d, const void *x, const float *lat, 
     if (rc) return rc;
     if (d->batch == 0) return SHTB200_OK;
     if (!x || !y || !stats) return fail(SHTB200_EINVAL, "null pointer");
+    if ((rc = check_values(*d, {x, y}, {weight, bias}, lat))) return rc;
     if (!aligned_alike(x, y)) return fail(SHTB200_EINVAL, "x and y must have the same address modulo 16");
     Launch l;
     if ((rc = plan(d, false, ws, ws_bytes, stats, &l))) return rc;
@@ -1596,6 +1604,7 @@ int group_norm_backward(const GroupNormDesc *d, const void *dy, const void *x, c
     if (rc) return rc;
     if (d->batch == 0) return fail(SHTB200_EINVAL, "an empty batch has no gradient to compute");
     if (!x || !dy || !stats) return fail(SHTB200_EINVAL, "null pointer");
+    if ((rc = check_values(*d, {x, dy, dx}, {weight, bias, dweight, dbias}, lat))) return rc;
     if (!aligned_alike(x, dy) || !aligned_alike(x, dx)) return fail(SHTB200_EINVAL, "x, dy and dx must have the same address modulo 16");
     Launch l;
     if ((rc = plan(d, true, ws, ws_bytes, stats, &l))) return rc;
