@@ -153,7 +153,7 @@ enum shtb200_norm { SHTB200_NORM_L2 = 0, SHTB200_NORM_INF = 1 };
 
 /*
  * Group normalisation of `batch` samples of `channels` fields on an nlat x nlon grid in `groups` groups of consecutive
- * channels, followed by a scale and shift per channel and an activation.  With a_k = lat_weights[k] >= 0 (any scale, not all 0; NULL: all 1):
+ * channels, followed by a scale and shift per channel and an activation.  With a_k = lat_weights[k] >= 0 (any scale, not all 0; values in rows of weight 0 are finite; NULL: all 1):
  *   mu = sum a x / sum a,  v = sum a (x - mu)^2 / sum a   over the channels and grid points of a group,
  *   y = act(weight_c (x - mu) / sqrt(v + eps) + bias_c).
  * `dtype` is the type of x, y, dy, dx (F32, BF16, F16), `param_dtype` that of weight, bias and their gradients.

@@ -5,19 +5,25 @@
 //     xh = (x - mu) r,  r = (v + eps)^(-1/2),  z = w_c xh + b_c,  y = act(z)
 // With g = dy act'(z), h = w_c g and q = a / sum a:
 //     db_c = sum g,  dw_c = sum g xh,  dx = r (h - q (sum h + xh sum h xh)).
-// A few operations per element: all of it is bound by memory, x (and dy) being read twice unless the second read finds them in L2.
+// A few operations per element: float32 is bound by memory, 16-bit fields by it and by the arithmetic of their 8 values a vector.  x (and dy) are read
+// from HBM twice, since a pass goes over the whole field before the next one begins.
 //
 // Two or three launches a direction: sums of chunks, their joining (in the second pass itself where that is little), the second pass.  The
 // work is cut into units (a sample, channels last; a plane, otherwise), units into chunks of pixels, a CTA each.  A chunk is read as one flat stream of
 // 16-byte vectors: with C' interleaved channels (C, or 1 for planes) and V values a vector, a thread that steps by a multiple of lcm(C', V)
 // values meets the same channels in every vector ("slots"), whatever C' is, and keeps their sums and parameters in registers.  The second
-// pass takes the last pieces of all chunks first: what the first has read last is still in L2.
+// pass takes the last pieces of all chunks first, since what the first has read last may still be in L2: of the 266 MB of 721x1440x64 float32 the counters
+// find 9 MB there, of the 133 MB of bf16 18 MB (backward, with twice as much read, nothing).
 //
 // All times below are device times on a B200 with a cold L2 (fields in HBM, copied at 6.56 TB/s).
 //
 // Sums for the variance are taken about a centre c per slot, (W, c, S1, S2) = (sum a, c, sum a (x - c), sum a (x - c)^2).  c begins as a value
-// of the field and is moved to the mean so far after 1, 2, 4, 8, ... rounds; fields whose level is far above their spread (pressures) or
-// that have a value far out lose nothing.  Chunks are joined in float64 as (W, K, mean - K, M2).
+// of the field (in a row that counts) and is moved to the mean so far after 1, 2, 4, 8, ... rounds; fields whose level is far above their spread
+// (pressures), that have a value far out, or whose rows weigh very differently lose nothing.  Chunks are joined in float64 as (W, K, mean - K, M2).
+//
+// What is held in float32: the sums of a thread and of the threads of a chunk (up to 2,000 terms one after the other; float64 would take twice the registers,
+// of which these loops are short), the slope and the activation, exponentials and reciprocals by the approximate instructions (2^-22).  Against 64 bits, 721x1440x64 and
+// 256x512x32 float32, root mean square: y 8e-8, dx 1.1e-7, dweight and dbias 1.2e-7 to 4e-7 of their own size (float64 sums: 8e-8 all).
 
 #include "common.cuh"
 
@@ -140,7 +146,8 @@ template <typename T, int ACT> __device__ __forceinline__ F2 act_value(F2 z) {
 }
 // The slope takes kSlopeScale z, which costs nothing where z is made from a scale and a shift, and comes divided by it again (OVER) where a scale
 // follows.  gelu'(z) = Phi(z) + z phi(z) = 1/2 + sign(z) (1/2 - e^(-a^2 / 2) (R(a) - a / sqrt(2 pi))), here with e^(-a^2 / 2) = 2^(-zs^2) and
-// R fitted (as above) in absolute error weighted by e^(-a^2 / 2): degree 5 with t = 1 / (1 + 0.28 a), 2.0e-7 over all z in float32 arithmetic.
+// R fitted (as above) in absolute error weighted by e^(-a^2 / 2): degree 5 with t = 1 / (1 + 0.28 a), 2.2e-7 over all z in float32 arithmetic.  Absolute,
+// since a slope is one term among those of size 1 in dx and in the sums; in the tail it is 7e-6 at z = -5, where the error is 0.7 % of it.
 template <int ACT> constexpr float kSlopeScale = ACT == SHTB200_ACT_GELU ? 0.84932180f : ACT == SHTB200_ACT_SILU ? 1.44269504f : 1.f;
 template <int ACT, bool OVER> __device__ __forceinline__ F2 act_slope(F2 zs) {
     constexpr float F = OVER ? 1.f / kSlopeScale<ACT> : 1.f;
@@ -353,9 +360,9 @@ __device__ __forceinline__ void advance(const GnArgs &a, Rows &r) {
 // Weights of the U vectors of a whole round, r and w moved on to the next one.  False, and nothing moved, where the vectors have to be taken one at
 // a time.
 // Planes look every vector's weight up, unless one lies across a row's end: a warp's round spans a third of a row of 1440 16-bit values, so a
-// branch for rounds within a row is taken both ways too often (721x1440x64 bf16, forward / backward: 85 / 136 us, with the branch 89 / 148).
-// Channels last a round spans a few points: those within a row share a weight, the others go one at a time (361x720x256 bf16: 87 / 134 us,
-// looked up 88 / 137).
+// branch for rounds within a row is taken both ways too often (721x1440x64 bf16, forward / backward: 85 / 134 us, with the branch 91 / 149).
+// Channels last a round spans a few points: those within a row share a weight, the others go one at a time (361x720x256 bf16: 90 / 136 us,
+// looked up 94 / 140).
 template <int U, bool PLANES> __device__ __forceinline__ bool round_weights(const GnArgs &a, int have, Rows &r, float &w, float (&wu)[U]) {
     if (have < U) return false;
     if (!a.lat || (!PLANES && r.col + U * a.step_px + r.over < a.nlon)) {  // all in one row, the next one too
@@ -671,12 +678,13 @@ __device__ __forceinline__ bool centre_on(uint4 raw, const F2 (&w)[kP<T>], float
 }
 
 constexpr int kUnroll = 2;
-template <typename T> constexpr int kStatsCtas = sizeof(T) == 4 ? 4 : 3;  // on an SM: 8 slots a thread spill at 4 (73 channels bf16 126 us, at 3 101); 4 slots do not
-using StatsFeed = Feed<1, kUnroll, 3>;  // (721x1440x73 bf16 channels last, forward: 101 us with 3 rounds, 103 with 2, 107 with 5)
+template <typename T> constexpr int kStatsCtas = sizeof(T) == 4 ? 4 : 3;  // on an SM: 8 slots a thread spill at 4 (73 channels bf16 119 us, at 3 103); 4 slots do not
+using StatsFeed = Feed<1, kUnroll, 3>;  // (721x1440x73 bf16 channels last, forward: 103 us with 3 rounds, 103 with 2, 107 with 5)
 
-// Sums of a chunk.  Bound by reading x in float32.  With 16-bit values a vector has twice the arithmetic: at 24 warps an SM 59 % of the issue slots are
-// taken and most warps wait for a result of their own (without the weights' multiplications it is no faster).
-// 721x1440x73 float32 planes, with the pass below: 165 us, 5.5 TB/s over two reads and a write.
+// Sums of a chunk.  Bound by reading x in float32.  With 16-bit values a vector has twice the arithmetic: at 24 warps an SM 60 % of the issue slots are
+// taken, and warps wait for a result of their own, or at the barriers at the end of a chunk, where few threads join its sums; of 73 channels three rows of 73
+// threads have vectors, so an eighth warp waits there from the start.  (Without the weights' multiplications it is no faster.)
+// 721x1440x73 float32 planes, with the pass below: 166 us, 5.5 TB/s over two reads and a write.
 
 template <typename T, bool PLANES> __global__ void __launch_bounds__(kThreads, kStatsCtas<T>) gn_stats_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kUnroll;
@@ -951,16 +959,16 @@ __global__ void __launch_bounds__(kThreads) gn_finish_stats_kernel(const __grid_
 }
 
 template <typename T, bool PLANES> constexpr int kApplyCtas = sizeof(T) == 2 && !PLANES ? 3 : 4;  // on an SM: 8 slots of different channels keep
-// more parameters than 4 CTAs leave registers for (361x720x256 bf16 forward 91 us, at 3 87; float32 gains from 4: 16x128x256x32 42 us, at 3 44)
+// more parameters than 4 CTAs leave registers for (721x1440x73 bf16 forward 106 us, at 3 103; 361x720x256 90 both; float32 gains from 4: 16x128x256x32 42 us, at 3 44)
 constexpr int kApplyUnroll = 2;
-using ApplyFeed = Feed<1, kApplyUnroll, 4>;  // (721x1440x73 float32 forward: 165 us with 4 rounds, 169 with 2, 165 with 6)
+using ApplyFeed = Feed<1, kApplyUnroll, 4>;  // (721x1440x73 float32 forward: 166 us with 4 rounds, 169 with 2, 164 with 6)
 
 // z = (x - m) sc + sh, the difference first, in every type: with the mean in the shift, the shift is rounded at |m| r, and where a group is constant or
 // nearly so r is up to eps^(-1/2) (a constant bf16 field of 101,376 came out 0.55 off, of 16-bit values exact as they are).  It costs 16-bit values a
-// subtraction and the registers of m: 361x720x256 bf16 channels last with gelu, forward / backward, 92 / 138 us, folded 87 / 135; planes 86 / 135, folded 84 / 134.
+// subtraction and the registers of m: 361x720x256 bf16 channels last with gelu, forward / backward, 91 / 139 us, folded 89 / 136; 721x1440x64 planes 87 / 135, folded 85 / 134.
 
 // y of a piece.  Bound by the write of y and the read of what L2 no longer holds of x; with 16-bit values and an activation by
-// its arithmetic too (721x1440x64 bf16 planes forward: 87 us with gelu and latitude weights, 73 without either).
+// its arithmetic too (721x1440x64 bf16 planes forward: 85 us with gelu and latitude weights, 73 without either).
 template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kThreads, kApplyCtas<T, PLANES>) gn_apply_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kApplyUnroll;
     extern __shared__ __align__(16) unsigned char gn_smem[];
@@ -1034,8 +1042,10 @@ template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kT
 // backward
 // ------------------------------------------------------------------------------------------------
 constexpr int kUnrollB = 2;
-constexpr int kBackwardCtas = 2;  // on an SM: what a thread keeps of 8 slots and the activation's constants spills at 3 (361x720x256 bf16 153 us, at 2 134)
-using BackwardFeed = Feed<2, kUnrollB, 2>;  // (deeper was slower: 721x1440x73 bf16 155 us with 2 rounds, 163 with 3, 167 with 4)
+// On an SM: what a thread keeps of 8 slots and the activation's constants spills at 3 (361x720x256 bf16 166 us, at 2 136).  Planes have one channel's
+// parameters and would take 3 without an activation, not with one (721x1440x64 bf16: none 122 us, at 2 128; gelu 138, at 2 134; float32 gelu 229, at 2 227).
+constexpr int kBackwardCtas = 2;
+using BackwardFeed = Feed<2, kUnrollB, 2>;  // (deeper was slower: 721x1440x73 bf16 155 us with 2 rounds, 166 with 3, 170 with 4; 721x1440x64 bf16 planes 134, 133 with 3)
 
 __device__ __forceinline__ void load_stats(const GnArgs &a, const Chunk &k, float4 *st) {
     if (a.cl)
@@ -1051,8 +1061,8 @@ template <typename T, int ACT> __device__ __forceinline__ float2 ragged_slope(co
 }
 
 // (sum g, sum g xh) of the channels of a chunk: the slope is evaluated here and again in the second pass, since storing g would cost a write and a
-// read of the field.  721x1440x64 float32 planes, with the pass below: 230 us, 5.8 TB/s over four reads and a write; with 16-bit values
-// the registers that 8 slots take leave 16 warps an SM, which wait for their own results (73 channels bf16: 153 us, 4.9 TB/s, 49 % of the issue slots).
+// read of the field.  721x1440x64 float32 planes, with the pass below: 227 us, 5.9 TB/s over four reads and a write; with 16-bit values
+// the registers that 8 slots take leave 16 warps an SM, which wait for their own results and at the barriers of a chunk's end (73 channels bf16: 155 us, 4.9 TB/s, 49 % of the issue slots).
 template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_sums_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kUnrollB;
     __shared__ __align__(16) F2 red[PLANES ? kWarps : P * kThreads];
@@ -1412,7 +1422,7 @@ template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kT
 // ------------------------------------------------------------------------------------------------
 constexpr int kMaxChannels = SHTB200_GROUP_NORM_MAX_CHANNELS;  // what a CTA keeps per channel or group has to fit into its shared memory
 // Partial results of a group up to which every CTA joins them itself, a warp a group, instead of a launch in between.  (256x512x32 float32,
-// forward: 30 us with the launch, 42 without, which a limit of 512 would choose; 16x128x256x32: 42 us without, 44 with, which 32 would.)
+// forward: 30 us with the launch, 40 without, which a limit of 512 would choose; 16x128x256x32: 42 us without, 44 with, which 32 would.)
 constexpr int kDirect = 128;
 
 int value_bytes(int dtype) { return dtype == SHTB200_F32 ? 4 : 2; }
@@ -1425,8 +1435,8 @@ struct Launch {
 };
 
 // Pieces of a chunk for the second pass: small ones follow what L2 holds more closely, large ones pay a CTA's start less often.  Forward, 721x1440x73
-// float32: 165 us, with whole chunks 172; 361x720x256 bf16: 87 us, with pieces of half the size 91 (backward, where they are twice as large:
-// 134 us, with half the size 142).
+// float32: 166 us, with whole chunks 172; 721x1440x64 bf16 planes 85 and 99; 361x720x256 bf16: 90 us, with pieces of half the size 92 (backward, where they
+// are twice as large: 136 us, with half the size 144).
 constexpr long long kPieceBytes = 128 << 10;
 constexpr int kMaxPieces = 4;
 
@@ -1459,7 +1469,7 @@ Launch geometry(const GroupNormDesc &d, bool backward) {
     a.step_rows = (int)(step_px / a.nlon);
     a.step_cols = (int)(step_px % a.nlon);
     // Chunks for the sums: one for every CTA that 148 SMs hold, but none under 16 KB, what a CTA does besides costing some microseconds (128x256x32 bf16
-    // forward and backward: 17.4 us each, with 4 KB 19.5 each, with 64 KB 19.5 and 21.5).
+    // forward and backward: 16.4 and 17.5 us, with 4 KB 19.5 and 19.4, with 64 KB 19.4 and 22.3).
     const int units = a.cl ? a.B : a.B * a.C, ctas = 148 * (backward ? kBackwardCtas : V == 4 ? kStatsCtas<float> : kStatsCtas<__half>);
     const long long unit_vecs = a.hw * a.cu / V, most = std::max<long long>(1, std::min<long long>(a.hw, unit_vecs / (kThreads * 4)));
     const long long n = std::min<long long>(most, std::max(1, ctas / units));

@@ -124,7 +124,7 @@ _guarded_gradients = once_differentiable(_gradients)
 
 
 # Where torch.compile traces, the call is a custom operator (as the transforms are), so that a network stays one graph.  Eager calls take the function
-# above instead, which is half the host time of such an operator.
+# above instead: host time of a small call 18 us, as an operator 30, of a small training step 119 and 200.
 _traced_call = functools.lru_cache(maxsize=256)(_call)
 
 
@@ -198,7 +198,11 @@ class GroupNormS2(nn.Module):
     The input is float32, bfloat16 or float16, in planes (contiguous) or channels last (``torch.channels_last``); both are read
     where they are, other strides are copied first.  The output has the input's type and layout; statistics, sums and the
     activation are float32 or wider whatever the type, under autocast too.  The parameters may have any of the three types.  The
-    gradients can be computed once (no second derivatives).
+    gradients can be computed once (no second derivatives).  Calls trace into one graph under ``torch.compile``; ``vmap`` and
+    forward-mode derivatives are not there.  ``lat_weights`` may be replaced by other float32 weights (nlat,) of at least 0: rows of weight 0
+    (whose values have to be finite) change no statistics and are normalised like the others.
+
+    A field is whole on its device: the tiles of ``distributed`` are not taken, since their statistics would be sums over the ranks.
 
     Calls may be captured into a CUDA graph.  A backward pass is captured only while no autograd graph of an eager step on the same
     parameters is alive (delete its loss first): torch accumulates gradients on the stream of that step, which ends the capture.
