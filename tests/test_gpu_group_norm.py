@@ -743,3 +743,37 @@ def test_errors_in_the_mean_square(shape, act, fmt):
     for name, o, e, bound in zip(("y", "dx", "dweight", "dbias"), _step(m, x, dy), _exact(m, x, dy)[0], (2.0**-20, 2.0**-20, 2.0**-19, 2.0**-19)):
         off = float((o.double() - e).norm() / e.norm())
         assert off <= bound, f"{name}: {off:.2e}"
+
+
+# channels, groups, nlat, nlon: one or a few vectors a thread, rows shorter than a vector, numbers of channels that do and do not divide a warp
+FAR_SHAPES = [(115, 23, 15, 31), (16, 4, 25, 51), (3, 3, 30, 1), (38, 38, 24, 49), (63, 21, 50, 72), (184, 23, 14, 28), (6, 3, 7, 3), (32, 2, 17, 36), (4, 4, 6, 12)]
+
+
+@pytest.mark.parametrize("fmt", ["planes", "last"])
+@pytest.mark.parametrize("dtype,level", [(torch.float32, 0.0), (torch.float32, 3.0e4), (torch.float16, 1.0e3)], ids=["f32", "f32_high", "f16"])
+@pytest.mark.parametrize("where", ["first", "pole", "last", "middle"])
+@pytest.mark.parametrize("shape", FAR_SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_one_point_far_out_in_small_fields(shape, where, dtype, level, fmt):
+    """A value of 3,000 spreads that may be all that a thread, a column or a channel's first slot has to begin with, at a pole with a hundredth of the others' weight or
+    less.  The bound is that of float32 above."""
+    C, G, H, W = shape
+    m = _module(G, C, H, W, activation="silu")
+    _parameters(m)
+    x, dy = _inputs((2, C, H, W), dtype, fmt, level=level)
+    i, j = {"first": (0, 0), "pole": (0, W // 2), "last": (H - 1, W - 1), "middle": (H // 2, W // 3)}[where]
+    x[:, :, i, j] += 3.0e3
+    _compare(_step(m, x, dy), *_exact(m, x, dy))
+
+
+@pytest.mark.parametrize("fmt", ["planes", "last"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows", [slice(0, 9), slice(5, 20), slice(0, 20, 2)], ids=str)
+def test_fill_values_in_rows_of_weight_zero(rows, dtype, fmt):
+    """The largest fill value in use (9.97e36), where the gradient is zero: it reaches neither the statistics nor a gradient."""
+    m = _module(2, 6, 20, 45, activation="silu")
+    _parameters(m)
+    m.lat_weights[rows] = 0.0
+    x, dy = _inputs((2, 6, 20, 45), dtype, fmt)
+    x[:, :, rows] = 9.96921e36
+    dy[:, :, rows] = 0.0
+    _compare(_step(m, x, dy), *_exact(m, x, dy))

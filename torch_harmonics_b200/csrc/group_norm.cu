@@ -31,7 +31,6 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
-#include <climits>
 #include <initializer_list>
 #include <map>
 #include <mutex>
@@ -544,13 +543,13 @@ struct Sums64 {
     }
 };
 
-// Sums over the threads of a column, K rounds of N pairs: pair i of column c at tot[i * kMaxCols + c].
-template <int K, int N> __device__ __forceinline__ void column_sums(const GnArgs &a, const Share &s, F2 (&v)[K * N], F2 *red, F2 *tot) {
+// Sums over the threads of a column, M pairs of each: pair i of column c at tot[i * kMaxCols + c].
+template <int M> __device__ __forceinline__ void column_sums(const GnArgs &a, const Share &s, F2 (&v)[M], F2 *red, F2 *tot) {
     int rep = s.rep, c = s.col, n = a.reps;
     if (a.windows == 1 && a.cols <= 32 && (a.cols & (a.cols - 1)) == 0) {  // whole columns in a warp: lanes first
         for (int o = 16; o >= a.cols; o >>= 1)
 #pragma unroll
-            for (int i = 0; i < K * N; ++i) {
+            for (int i = 0; i < M; ++i) {
                 F2 u;
                 u.v = __shfl_xor_sync(0xffffffffu, v[i].v, o);
                 v[i] = add2(v[i], u);
@@ -559,21 +558,18 @@ template <int K, int N> __device__ __forceinline__ void column_sums(const GnArgs
         rep = c < a.cols ? (int)(threadIdx.x >> 5) : kThreads;
         n = kWarps;
     }
+    if (rep < n)
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        if (rep < n)
-#pragma unroll
-            for (int i = 0; i < N; ++i) red[i * kThreads + rep * a.win_cols + c] = v[k * N + i];
-        __syncthreads();
-        for (int o = threadIdx.x; o < N * a.win_cols; o += kThreads) {
-            const int i = (int)((unsigned)o / (unsigned)a.win_cols), col = o - i * a.win_cols;
-            const F2 *p = red + i * kThreads + col;
-            F2 t = p[0];
-            for (int r = 1; r < n; ++r) t = add2(t, p[r * a.win_cols]);
-            tot[(k * N + i) * kMaxCols + col] = t;
-        }
-        __syncthreads();
+        for (int i = 0; i < M; ++i) red[i * kThreads + rep * a.win_cols + c] = v[i];
+    __syncthreads();
+    for (int o = threadIdx.x; o < M * a.win_cols; o += kThreads) {
+        const int i = (int)((unsigned)o / (unsigned)a.win_cols), col = o - i * a.win_cols;
+        const F2 *p = red + i * kThreads + col;
+        F2 t = p[0];
+        for (int r = 1; r < n; ++r) t = add2(t, p[r * a.win_cols]);
+        tot[i * kMaxCols + col] = t;
     }
+    __syncthreads();
 }
 __device__ __forceinline__ float half_of(const F2 *tot, int pair, int col, int h) { return reinterpret_cast<const float *>(tot + pair * kMaxCols + col)[h]; }
 
@@ -688,10 +684,9 @@ using StatsFeed = Feed<1, kUnroll, 3>;  // (721x1440x73 bf16 channels last, forw
 
 template <typename T, bool PLANES> __global__ void __launch_bounds__(kThreads, kStatsCtas<T>) gn_stats_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kUnroll;
-    __shared__ __align__(16) F2 red[P * kThreads];
-    __shared__ __align__(16) F2 tot[PLANES ? kWarps * 2 : 3 * P * kMaxCols];
-    __shared__ float centre[PLANES ? V : V * kMaxCols];
-    constexpr int kPitch = PLANES ? 1 : kMaxCols;
+    __shared__ __align__(16) F2 red[(PLANES ? 1 : 2) * P * kThreads];
+    __shared__ __align__(16) F2 tot[PLANES ? kWarps * 2 : 4 * P * kMaxCols];  // of the columns: W, W (mean - centre), S1, S2
+    __shared__ __align__(16) F2 centre[PLANES ? 1 : P * kMaxCols];
     // weights of a slot beyond its thread's common ones, where vectors lie across rows: rare, and registers are short
     F2(*extra)[kThreads] = reinterpret_cast<F2(*)[kThreads]>(red);
     extern __shared__ __align__(16) unsigned char gn_smem[];
@@ -789,67 +784,49 @@ template <typename T, bool PLANES> __global__ void __launch_bounds__(kThreads, k
                 }
             }
         }
-        // all threads of a column: about the centre of its first thread, then added (planes: of the first slot of all)
-        F2 z[3 * P];  // W, S1, S2
-        bool lost = false;
+        // All threads of a column about their common mean, then added (planes: all slots of all threads).  The mean of one thread would not do as the
+        // centre of all: it may hold little but a value at the pole, far out, whose weight is a ten thousandth of the others'.
+        // (It is taken relative to the first thread's, so that the mean of a constant is that constant.)
+        F2 z[P];  // W
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            z[p] = add2(extra[p][threadIdx.x], f2(W));
-            const float2 v = split(c[p]), counted = split(z[p]);
-            if (s.rep == 0) {
-                centre[(2 * p) * kPitch + s.col] = v.x;
-                centre[(2 * p + 1) * kPitch + s.col] = v.y;
-                if (!PLANES || p == 0) lost |= counted.x == 0.f || (!PLANES && counted.y == 0.f);
-            }
-        }
-        // (where that one has met only rows that do not count: of the first that has met another)
-        if (__syncthreads_or(lost && s.count)) {
-            int *first = reinterpret_cast<int *>(tot);
-            for (int i = threadIdx.x; i < (PLANES ? 1 : V * kMaxCols); i += kThreads) first[i] = INT_MAX;
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float2 counted = split(z[i / 2]);
-                if (s.count && (i & 1 ? counted.y : counted.x) > 0.f) atomicMin(first + (PLANES ? 0 : i * kMaxCols + s.col), PLANES ? s.rep * V + i : s.rep);
-            }
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float2 v = split(c[i / 2]);
-                if (s.count && first[PLANES ? 0 : i * kMaxCols + s.col] == (PLANES ? s.rep * V + i : s.rep)) centre[(PLANES ? 0 : i) * kPitch + s.col] = i & 1 ? v.y : v.x;
-            }
-            __syncthreads();
-        }
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-            const F2 c0 = PLANES ? f2(centre[0]) : f2(centre[(2 * p) * kPitch + s.col], centre[(2 * p + 1) * kPitch + s.col]);
-            if (s.count) recentre(z[p], sub2(c0, c[p]), q[p], q[P + p]);
-            z[P + p] = q[p];
-            z[2 * P + p] = q[P + p];
-        }
+        for (int p = 0; p < P; ++p) z[p] = add2(extra[p][threadIdx.x], f2(W));
         if constexpr (PLANES) {
-            float v[3];
+            F2 *first = tot, *second = tot + kWarps;  // (W, mean) and (S1, S2) of every warp
+            const int warp = threadIdx.x >> 5;
+            auto slots = [](const F2 *v) {
+                F2 t = v[0];
 #pragma unroll
-            for (int i = 0; i < 3; ++i) {
-                F2 t = z[i * P];
-#pragma unroll
-                for (int p = 1; p < P; ++p) t = add2(t, z[i * P + p]);
+                for (int p = 1; p < P; ++p) t = add2(t, v[p]);
                 const float2 h = split(t);
-                v[i] = h.x + h.y;
-                for (int o = 16; o; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-            }
-            float *w = reinterpret_cast<float *>(tot);
-            if ((threadIdx.x & 31) == 0)
+                return h.x + h.y;
+            };
+            auto lanes = [](float v) {
+                for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                return v;
+            };
+            F2 t[P];
+            const float w = lanes(slots(z)), inv = w > 0.f ? __fdividef(1.f, w) : 0.f;
+            const float lane0 = __shfl_sync(0xffffffffu, split(z[0]).x > 0.f ? split(c[0]).x : 0.f, 0);
 #pragma unroll
-                for (int i = 0; i < 3; ++i) w[i * kWarps + (threadIdx.x >> 5)] = v[i];
+            for (int p = 0; p < P; ++p) t[p] = fma2(mul2(z[p], f2(inv)), sub2(c[p], f2(lane0)), mul2(q[p], f2(inv)));
+            const float mean = lane0 + lanes(slots(t));
+            if ((threadIdx.x & 31) == 0) first[warp] = f2(w, mean);
+            __syncthreads();
+            float all = 0.f, off = 0.f;
+            for (int n = 0; n < kWarps; ++n) all += split(first[n]).x;
+            const float part = all > 0.f ? __fdividef(1.f, all) : 0.f, warp0 = split(first[0]).x > 0.f ? split(first[0]).y : 0.f;
+            for (int n = 0; n < kWarps; ++n) off = fmaf(split(first[n]).x * part, split(first[n]).y - warp0, off);
+            const float c0 = warp0 + off;
+            if (s.count)
+#pragma unroll
+                for (int p = 0; p < P; ++p) recentre(z[p], sub2(f2(c0), c[p]), q[p], q[P + p]);
+            const float S1 = lanes(slots(q)), S2 = lanes(slots(q + P));
+            if ((threadIdx.x & 31) == 0) second[warp] = f2(S1, S2);
             __syncthreads();
             if (threadIdx.x == 0) {
-#pragma unroll
-                for (int i = 0; i < 3; ++i) {
-                    v[i] = w[i * kWarps];
-                    for (int n = 1; n < kWarps; ++n) v[i] += w[i * kWarps + n];
-                }
-                Moments m = moments(v[0], centre[0], v[1], v[2]);
+                F2 v = second[0];
+                for (int n = 1; n < kWarps; ++n) v = add2(v, second[n]);
+                Moments m = moments(all, c0, split(v).x, split(v).y);
                 for (int i = 0; i < 2 * V; ++i) {  // the values outside the vectors
                     const int e = ragged<T>(k, i);
                     if (e < 0) break;
@@ -858,7 +835,26 @@ template <typename T, bool PLANES> __global__ void __launch_bounds__(kThreads, k
                 out[0] = make_float4(m.W, m.K, m.m, m.M2);
             }
         } else {
-            column_sums<3, P>(a, s, z, red, tot);
+            F2 t[2 * P];
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                const float2 counted = split(z[p]), v = split(c[p]);
+                if (s.rep == 0) centre[p * kMaxCols + s.col] = f2(counted.x > 0.f ? v.x : 0.f, counted.y > 0.f ? v.y : 0.f);
+            }
+            __syncthreads();  // (the columns are added where `extra` was, too)
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                t[p] = z[p];
+                t[P + p] = fma2(z[p], sub2(c[p], centre[p * kMaxCols + s.col]), q[p]);
+            }
+            column_sums(a, s, t, red, tot);
+            if (s.count)
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    const F2 c0 = fma2(tot[(P + p) * kMaxCols + s.col], reciprocal(tot[p * kMaxCols + s.col]), centre[p * kMaxCols + s.col]);
+                    recentre(z[p], sub2(c0, c[p]), q[p], q[P + p]);
+                }
+            column_sums(a, s, q, red, tot + 2 * P * kMaxCols);
             // groups: a few lanes each go through its channels' slots in this window
             const int period = a.cols * V, slots = a.cgu * a.dup, shift = k.head % a.cu, L = a.lanes;
             const int sub = threadIdx.x & (L - 1), lo = win * a.win_cols * V, hi = min(lo + a.win_cols * V, period);
@@ -873,7 +869,9 @@ template <typename T, bool PLANES> __global__ void __launch_bounds__(kThreads, k
                         e += again * a.cu;
                         if (e >= lo && e < hi) {
                             const int col = (e - lo) / V, i2 = (e - lo) % V;
-                            join(m, moments(half_of(tot, i2 / 2, col, i2 & 1), centre[i2 * kMaxCols + col], half_of(tot, P + i2 / 2, col, i2 & 1), half_of(tot, 2 * P + i2 / 2, col, i2 & 1)));
+                            const float Wc = half_of(tot, i2 / 2, col, i2 & 1), inv = Wc > 0.f ? __fdividef(1.f, Wc) : 0.f;
+                            const float c0 = fmaf(half_of(tot, P + i2 / 2, col, i2 & 1), inv, half_of(centre, i2 / 2, col, i2 & 1));  // (as above, to the bit)
+                            join(m, moments(Wc, c0, half_of(tot, 2 * P + i2 / 2, col, i2 & 1), half_of(tot, 3 * P + i2 / 2, col, i2 & 1)));
                         }
                     }
                 for (int o = L / 2; o; o >>= 1) {
@@ -1065,7 +1063,7 @@ template <typename T, int ACT> __device__ __forceinline__ float2 ragged_slope(co
 // the registers that 8 slots take leave 16 warps an SM, which wait for their own results and at the barriers of a chunk's end (73 channels bf16: 155 us, 4.9 TB/s, 49 % of the issue slots).
 template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_sums_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kUnrollB;
-    __shared__ __align__(16) F2 red[PLANES ? kWarps : P * kThreads];
+    __shared__ __align__(16) F2 red[PLANES ? kWarps : 2 * P * kThreads];
     __shared__ __align__(16) F2 tot[PLANES ? 1 : 2 * P * kMaxCols];
     extern __shared__ __align__(16) unsigned char gn_smem[];
     float4 *st = reinterpret_cast<float4 *>(gn_smem + BackwardFeed::bytes);
@@ -1151,7 +1149,7 @@ template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kT
                 out[0] = make_float2(t.x, st[0].z * fmaf(-st[0].y, t.x, t.y));  // sum g (x - m) -> sum g xh
             }
         } else {
-            column_sums<2, P>(a, s, q, red, tot);
+            column_sums(a, s, q, red, tot);
             const int period = a.cols * V, lo = win * a.win_cols * V, hi = min(lo + a.win_cols * V, period), shift = k.head % a.cu;
             for (int c = threadIdx.x; c < a.cu; c += kThreads) {
                 float2 t = acc[c];
