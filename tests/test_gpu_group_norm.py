@@ -766,6 +766,20 @@ def test_one_point_far_out_in_small_fields(shape, where, dtype, level, fmt):
 
 
 @pytest.mark.parametrize("fmt", ["planes", "last"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16], ids=["f32", "f16"])
+@pytest.mark.parametrize("shape", FAR_SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_rows_of_very_different_weight(shape, dtype, fmt):
+    """Weights between 1e-6 and 1, neighbours too, with a value far out in the lightest row."""
+    C, G, H, W = shape
+    m = _module(G, C, H, W, activation="gelu")
+    _parameters(m)
+    m.lat_weights[:] = torch.exp(-14 * torch.rand(H, device="cuda", generator=torch.Generator(device="cuda").manual_seed(H)))
+    x, dy = _inputs((2, C, H, W), dtype, fmt, level=10.0)
+    x[:, :, int(m.lat_weights.argmin()), W // 2] += 3.0e3
+    _compare(_step(m, x, dy), *_exact(m, x, dy))
+
+
+@pytest.mark.parametrize("fmt", ["planes", "last"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("rows", [slice(0, 9), slice(5, 20), slice(0, 20, 2)], ids=str)
 def test_fill_values_in_rows_of_weight_zero(rows, dtype, fmt):

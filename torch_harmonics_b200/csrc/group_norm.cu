@@ -485,10 +485,11 @@ __device__ __forceinline__ void join(Moments &a, const Moments &b) {
         a = b;
         return;
     }
-    const float W = a.W + b.W, f = __fdividef(b.W, W), d = (b.K - a.K) + (b.m - a.m);
-    a.m = fmaf(d, f, a.m);
-    a.M2 += fmaf(d * d, a.W * f, b.M2);
-    a.W = W;
+    // (from the mean of the part that weighs more: the other's may be far from it, and the rounding of f would move the mean by as much of that)
+    const bool swap = b.W > a.W;
+    const Moments heavy = swap ? b : a, light = swap ? a : b;
+    const float W = a.W + b.W, f = __fdividef(light.W, W), d = (light.K - heavy.K) + (light.m - heavy.m);
+    a = {W, heavy.K, fmaf(d, f, heavy.m), heavy.M2 + fmaf(d * d, heavy.W * f, light.M2)};
     normalise(a);
 }
 
@@ -687,7 +688,7 @@ template <typename T, bool PLANES> __global__ void __launch_bounds__(kThreads, k
     __shared__ __align__(16) F2 red[(PLANES ? 1 : 2) * P * kThreads];
     __shared__ __align__(16) F2 tot[PLANES ? kWarps * 2 : 4 * P * kMaxCols];  // of the columns: W, W (mean - centre), S1, S2
     __shared__ __align__(16) F2 centre[PLANES ? 1 : P * kMaxCols];
-    // weights of a slot beyond its thread's common ones, where vectors lie across rows: rare, and registers are short
+    // weights of a slot in the vectors that lie across rows, beside those that all slots share: rare, and registers are short
     F2(*extra)[kThreads] = reinterpret_cast<F2(*)[kThreads]>(red);
     extern __shared__ __align__(16) unsigned char gn_smem[];
     Moments *acc = reinterpret_cast<Moments *>(gn_smem + StatsFeed::bytes);
@@ -763,10 +764,11 @@ template <typename T, bool PLANES> __global__ void __launch_bounds__(kThreads, k
                             if (open || mixed || w > W) open = centre_on<T>(raw[u], wp, W, extra, c, q);
                             if (mixed)
 #pragma unroll
-                                for (int p = 0; p < P; ++p) extra[p][threadIdx.x] = add2(extra[p][threadIdx.x], sub2(wp[p], f2(w)));
+                                for (int p = 0; p < P; ++p) extra[p][threadIdx.x] = add2(extra[p][threadIdx.x], wp[p]);
+                            else
+                                W += w;
                             unpack(raw[u], v, T());
                             accumulate<T>(v, c, q, wp);
-                            W += w;
                             if (a.lat) {
                                 advance(a, r);
                                 w = __ldg(a.lat + min(r.row, a.nlat - 1));
