@@ -791,3 +791,17 @@ def test_fill_values_in_rows_of_weight_zero(rows, dtype, fmt):
     x[:, :, rows] = 9.96921e36
     dy[:, :, rows] = 0.0
     _compare(_step(m, x, dy), *_exact(m, x, dy))
+
+
+@pytest.mark.parametrize("fmt", ["planes", "last"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("nlon", [541, 1080, 2160])
+@pytest.mark.parametrize("column", [5, 400])
+def test_heavy_rows_after_light_ones(column, nlon, dtype, fmt):
+    """The same in fields of many vectors a thread: every other row weighs a millionth and has a value far out, the next row follows at any of a thread's rounds."""
+    m = _module(2, 4, 90, nlon, activation="silu")
+    m.lat_weights[0::2] = 1.0e-6
+    m.lat_weights[1::2] = 1.0
+    x, dy = _inputs((1, 4, 90, nlon), dtype, fmt)
+    x[:, :, 0::2, column] += 1.0e7
+    _compare(_step(m, x, dy), *_exact(m, x, dy))

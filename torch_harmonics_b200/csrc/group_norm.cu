@@ -730,7 +730,7 @@ template <typename T, bool PLANES> __global__ void __launch_bounds__(kThreads, k
                 // The first centre: of the first round that counts, the vector that counts most (a value at the pole, far out, is none for rows of a
                 // hundred times its weight, and one in a row that does not count is none at all).
                 if (round_weights<U, PLANES>(a, have, r, w, wu)) {
-                    if (open) {
+                    if (open || wu[U - 1] > W) {
                         const bool last = wu[U - 1] >= wu[0];
                         const float most = last ? wu[U - 1] : wu[0];
                         F2 wp[P];
