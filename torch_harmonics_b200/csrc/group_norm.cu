@@ -13,7 +13,7 @@
 // 16-byte vectors: with C' interleaved channels (C, or 1 for planes) and V values a vector, a thread that steps by a multiple of lcm(C', V)
 // values meets the same channels in every vector ("slots"), whatever C' is, and keeps their sums and parameters in registers.  The second
 // pass takes the last pieces of all chunks first, since what the first has read last may still be in L2: of the 266 MB of 721x1440x64 float32 the counters
-// find 9 MB there, of the 133 MB of bf16 18 MB (backward, with twice as much read, nothing).
+// find 9 MB there, of the 133 MB of bf16 19 MB (backward, with twice as much read, nothing).
 //
 // All times below are device times on a B200 with a cold L2 (fields in HBM, copied at 6.56 TB/s).
 //
@@ -359,9 +359,10 @@ __device__ __forceinline__ void advance(const GnArgs &a, Rows &r) {
 // Weights of the U vectors of a whole round, r and w moved on to the next one.  False, and nothing moved, where the vectors have to be taken one at
 // a time.
 // Planes look every vector's weight up, unless one lies across a row's end: a warp's round spans a third of a row of 1440 16-bit values, so a
-// branch for rounds within a row is taken both ways too often (721x1440x64 bf16, forward / backward: 85 / 134 us, with the branch 91 / 149).
-// Channels last a round spans a few points: those within a row share a weight, the others go one at a time (361x720x256 bf16: 90 / 136 us,
-// looked up 94 / 140).
+// branch for rounds within a row is taken both ways too often (721x1440x64 bf16, forward / backward: 86 / 135 us, with the branch 92 / 151; 721x1440x73
+// float32 forward 161, with it 159).
+// Channels last a round spans a few points: those within a row share a weight, the others go one at a time (361x720x256 bf16: 92 / 138 us,
+// looked up 94 / 142).
 template <int U, bool PLANES> __device__ __forceinline__ bool round_weights(const GnArgs &a, int have, Rows &r, float &w, float (&wu)[U]) {
     if (have < U) return false;
     if (!a.lat || (!PLANES && r.col + U * a.step_px + r.over < a.nlon)) {  // all in one row, the next one too
@@ -675,13 +676,13 @@ __device__ __forceinline__ bool centre_on(uint4 raw, const F2 (&w)[kP<T>], float
 }
 
 constexpr int kUnroll = 2;
-template <typename T> constexpr int kStatsCtas = sizeof(T) == 4 ? 4 : 3;  // on an SM: 8 slots a thread spill at 4 (73 channels bf16 119 us, at 3 103); 4 slots do not
-using StatsFeed = Feed<1, kUnroll, 3>;  // (721x1440x73 bf16 channels last, forward: 103 us with 3 rounds, 103 with 2, 107 with 5)
+template <typename T> constexpr int kStatsCtas = sizeof(T) == 4 ? 4 : 3;  // on an SM: 8 slots a thread spill at 4 (73 channels bf16 122 us, at 3 103); 4 slots do not
+using StatsFeed = Feed<1, kUnroll, 3>;  // (721x1440x73 bf16 channels last, forward: 103 us with 3 rounds, 104 with 2, 115 with 5)
 
-// Sums of a chunk.  Bound by reading x in float32.  With 16-bit values a vector has twice the arithmetic: at 24 warps an SM 60 % of the issue slots are
+// Sums of a chunk.  Bound by reading x in float32.  With 16-bit values a vector has twice the arithmetic: at 24 warps an SM 61 % of the issue slots are
 // taken, and warps wait for a result of their own, or at the barriers at the end of a chunk, where few threads join its sums; of 73 channels three rows of 73
 // threads have vectors, so an eighth warp waits there from the start.  (Without the weights' multiplications it is no faster.)
-// 721x1440x73 float32 planes, with the pass below: 166 us, 5.5 TB/s over two reads and a write.
+// 721x1440x73 float32 planes, with the pass below: 161 us, 5.7 TB/s over two reads and a write.
 
 template <typename T, bool PLANES> __global__ void __launch_bounds__(kThreads, kStatsCtas<T>) gn_stats_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kUnroll;
@@ -959,16 +960,16 @@ __global__ void __launch_bounds__(kThreads) gn_finish_stats_kernel(const __grid_
 }
 
 template <typename T, bool PLANES> constexpr int kApplyCtas = sizeof(T) == 2 && !PLANES ? 3 : 4;  // on an SM: 8 slots of different channels keep
-// more parameters than 4 CTAs leave registers for (721x1440x73 bf16 forward 106 us, at 3 103; 361x720x256 90 both; float32 gains from 4: 16x128x256x32 42 us, at 3 44)
+// more parameters than 4 CTAs leave registers for (721x1440x73 bf16 forward 106 us, at 3 103; 361x720x256 92 both; float32 gains from 4: 16x128x256x32 42 us, at 3 43)
 constexpr int kApplyUnroll = 2;
-using ApplyFeed = Feed<1, kApplyUnroll, 4>;  // (721x1440x73 float32 forward: 166 us with 4 rounds, 169 with 2, 164 with 6)
+using ApplyFeed = Feed<1, kApplyUnroll, 4>;  // (721x1440x73 float32 forward: 161 us with 4 rounds, 163 with 2, 158 with 6)
 
 // z = (x - m) sc + sh, the difference first, in every type: with the mean in the shift, the shift is rounded at |m| r, and where a group is constant or
 // nearly so r is up to eps^(-1/2) (a constant bf16 field of 101,376 came out 0.55 off, of 16-bit values exact as they are).  It costs 16-bit values a
-// subtraction and the registers of m: 361x720x256 bf16 channels last with gelu, forward / backward, 91 / 139 us, folded 89 / 136; 721x1440x64 planes 87 / 135, folded 85 / 134.
+// subtraction and the registers of m: 361x720x256 bf16 channels last with gelu, forward / backward, 92 / 138 us, folded 89 / 135; 721x1440x64 planes 86 / 135, folded 85 / 134.
 
 // y of a piece.  Bound by the write of y and the read of what L2 no longer holds of x; with 16-bit values and an activation by
-// its arithmetic too (721x1440x64 bf16 planes forward: 85 us with gelu and latitude weights, 73 without either).
+// its arithmetic too (721x1440x64 bf16 planes forward: 86 us with gelu and latitude weights, 72 without either).
 template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kThreads, kApplyCtas<T, PLANES>) gn_apply_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kApplyUnroll;
     extern __shared__ __align__(16) unsigned char gn_smem[];
@@ -1042,10 +1043,10 @@ template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kT
 // backward
 // ------------------------------------------------------------------------------------------------
 constexpr int kUnrollB = 2;
-// On an SM: what a thread keeps of 8 slots and the activation's constants spills at 3 (361x720x256 bf16 166 us, at 2 136).  Planes have one channel's
-// parameters and would take 3 without an activation, not with one (721x1440x64 bf16: none 122 us, at 2 128; gelu 138, at 2 134; float32 gelu 229, at 2 227).
+// On an SM: what a thread keeps of 8 slots and the activation's constants spills at 3 (361x720x256 bf16 167 us, at 2 138).  Planes have one channel's
+// parameters and would take 3 without an activation, not with one (721x1440x64 bf16: none 121 us, at 2 127; gelu 139, at 2 135; float32 gelu 231, at 2 226).
 constexpr int kBackwardCtas = 2;
-using BackwardFeed = Feed<2, kUnrollB, 2>;  // (deeper was slower: 721x1440x73 bf16 155 us with 2 rounds, 166 with 3, 170 with 4; 721x1440x64 bf16 planes 134, 133 with 3)
+using BackwardFeed = Feed<2, kUnrollB, 2>;  // (deeper was slower: 721x1440x73 bf16 155 us with 2 rounds, 165 with 3, 170 with 4; 721x1440x64 bf16 planes 135 with 2 and 3)
 
 __device__ __forceinline__ void load_stats(const GnArgs &a, const Chunk &k, float4 *st) {
     if (a.cl)
@@ -1061,7 +1062,7 @@ template <typename T, int ACT> __device__ __forceinline__ float2 ragged_slope(co
 }
 
 // (sum g, sum g xh) of the channels of a chunk: the slope is evaluated here and again in the second pass, since storing g would cost a write and a
-// read of the field.  721x1440x64 float32 planes, with the pass below: 227 us, 5.9 TB/s over four reads and a write; with 16-bit values
+// read of the field.  721x1440x64 float32 planes, with the pass below: 226 us, 5.9 TB/s over four reads and a write; with 16-bit values
 // the registers that 8 slots take leave 16 warps an SM, which wait for their own results and at the barriers of a chunk's end (73 channels bf16: 155 us, 4.9 TB/s, 49 % of the issue slots).
 template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kThreads, kBackwardCtas) gn_sums_kernel(const __grid_constant__ GnArgs a) {
     constexpr int V = kV<T>, P = kP<T>, U = kUnrollB;
@@ -1422,7 +1423,7 @@ template <typename T, int ACT, bool PLANES> __global__ void __launch_bounds__(kT
 // ------------------------------------------------------------------------------------------------
 constexpr int kMaxChannels = SHTB200_GROUP_NORM_MAX_CHANNELS;  // what a CTA keeps per channel or group has to fit into its shared memory
 // Partial results of a group up to which every CTA joins them itself, a warp a group, instead of a launch in between.  (256x512x32 float32,
-// forward: 30 us with the launch, 40 without, which a limit of 512 would choose; 16x128x256x32: 42 us without, 44 with, which 32 would.)
+// forward: 29 us with the launch, 39 without, which a limit of 512 would choose; 16x128x256x32: 42 us without, 43 with, which 32 would.)
 constexpr int kDirect = 128;
 
 int value_bytes(int dtype) { return dtype == SHTB200_F32 ? 4 : 2; }
@@ -1435,8 +1436,8 @@ struct Launch {
 };
 
 // Pieces of a chunk for the second pass: small ones follow what L2 holds more closely, large ones pay a CTA's start less often.  Forward, 721x1440x73
-// float32: 166 us, with whole chunks 172; 721x1440x64 bf16 planes 85 and 99; 361x720x256 bf16: 90 us, with pieces of half the size 92 (backward, where they
-// are twice as large: 136 us, with half the size 144).
+// float32: 161 us, with whole chunks 166; 721x1440x64 bf16 planes 86 and 100; 361x720x256 bf16: 92 us, with pieces of half the size 94 (backward, where they
+// are twice as large: 138 us, with half the size 145).
 constexpr long long kPieceBytes = 128 << 10;
 constexpr int kMaxPieces = 4;
 
@@ -1469,7 +1470,7 @@ Launch geometry(const GroupNormDesc &d, bool backward) {
     a.step_rows = (int)(step_px / a.nlon);
     a.step_cols = (int)(step_px % a.nlon);
     // Chunks for the sums: one for every CTA that 148 SMs hold, but none under 16 KB, what a CTA does besides costing some microseconds (128x256x32 bf16
-    // forward and backward: 16.4 and 17.5 us, with 4 KB 19.5 and 19.4, with 64 KB 19.4 and 22.3).
+    // forward and backward: 16.0 and 16.4 us, with 4 KB 19.6 and 18.4, with 64 KB 18.2 and 20.7).
     const int units = a.cl ? a.B : a.B * a.C, ctas = 148 * (backward ? kBackwardCtas : V == 4 ? kStatsCtas<float> : kStatsCtas<__half>);
     const long long unit_vecs = a.hw * a.cu / V, most = std::max<long long>(1, std::min<long long>(a.hw, unit_vecs / (kThreads * 4)));
     const long long n = std::min<long long>(most, std::max(1, ctas / units));
